@@ -44,6 +44,7 @@
 #include "common.h"
 #include "dev.cuh"
 #include "gemm_tc.cuh"
+#include "ptx.cuh"
 
 namespace vb::tc {
 
@@ -56,6 +57,7 @@ using vb::d::rnd;
 using vb::d::seg_add;
 using vb::d::seg_record;
 using vb::d::to_f;
+using namespace vb::ptx;
 
 constexpr int BM = 128, BK = 64;
 constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
@@ -90,44 +92,6 @@ struct Params {
 constexpr int kLnNone = 0, kLnStats = 1, kLnFold = 2;
 constexpr int kMaxSegs = 16;  // records per row a folded GEMM reads (C <= 2048)
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// ... with acquire at cluster scope (for arrivals that carry another CTA's shared-memory writes)
-__device__ __forceinline__ bool mbar_test_cl(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 // Bounded wait for the phase of parity `parity`. Returns false on timeout (after raising the CTA's
 // abort flag and the device error flag) or when another role already aborted.
 template <bool CL = false>
@@ -153,14 +117,6 @@ __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
             atomicExch(&g_error, 2);
             return;
         }
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
 }
 
 // Shared-memory matrix descriptor: K-major tile, 128-byte swizzle, 8-row groups 1024 bytes apart.
@@ -190,42 +146,9 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b,
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
 // ---- CTA pairs (cta_group::2): the MMA of a cluster of two CTAs on SMs of one TPC computes a
 // 256-row tile; each CTA holds its 128 rows of A and half of the BN rows of B in its own shared
 // memory, and its 128 rows of the accumulator in its own TMEM.
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// shared::cluster address of the variable at shared::cta address `a` in the cluster's CTA `rank`
-__device__ __forceinline__ uint32_t mapa(uint32_t a, uint32_t rank) {
-    uint32_t d;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(rank));
-    return d;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
-}
-// TMA tile load into this CTA's shared memory whose bytes complete on the barrier at `bar_cluster`
-// (the pair leader's); no multicast.
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster)
-        : "memory");
-}
 __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -233,69 +156,6 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-// completion of the pair's MMAs issued so far, arriving on the barrier at the same offset in both CTAs
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
-        "h"(uint16_t(3))
-        : "memory");
-}
-// ... and on this CTA's barrier only
-__device__ __forceinline__ void mma_commit_pair_local(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// tcgen05.ld of 32 consecutive TMEM columns of this warp's 32 lanes, without waiting; tmem_wait32
-// waits for every load of the thread and hands the registers on (they are in-out operands of the
-// wait, so no use of them can be scheduled before it).
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
-}
-
-// x + h (h an fp16 value, widened exactly): the sm_100 mixed-precision add, one instruction per element.
-__device__ __forceinline__ float2 add_h2(uint32_t h2, float2 x) {
-    float2 d;
-    asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
-        "add.rn.f32.f16 %0, lo, %3;\n\tadd.rn.f32.f16 %1, hi, %4;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "r"(h2), "f"(x.x), "f"(x.y));
-    return d;
-}
-// Two fp32 values rounded to fp16 and packed (low half = x.x).
-__device__ __forceinline__ uint32_t pack_h2(float2 x) {
-    const __half2 h = __floats2half2_rn(x.x, x.y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Shared memory: the A/W stage ring, then per epilogue warp two 2 KB output staging buffers, then the
 // mbarriers, the TMEM address and abort flag, and the ring of tile indices (dynamic tile order).
 template <int BN, int STAGES, int EPI, bool PAIR> struct Layout {
@@ -308,48 +168,6 @@ template <int BN, int STAGES, int EPI, bool PAIR> struct Layout {
     static constexpr int kSmem = 1024 + kTiles + kOut + kBars + 16 + 4 * kRing;  // 1024: alignment slack
     static_assert(kSmem <= 232448, "shared memory over the 227 KB per-CTA limit");
 };
-
-// GELU for the fp16 path: x * Phi(x), Phi from the erf approximation of Abramowitz & Stegun,
-// Handbook of Mathematical Functions, formula 7.1.26 (|error of erf| <= 1.5e-7), written as
-// Phi(x) = 1 - q (x >= 0), q (x < 0) with q = P(t) exp(-z^2) / 2, z = |x| / sqrt(2), so the left tail
-// has no cancellation. Checked against the erff-based GELU by the tests.
-// Two values at a time with packed fp32 operations; q's factor 1/2 is folded into the polynomial's
-// coefficients (exact: a power of two); exp(-z^2) = 2^(-z^2 log2 e) and the reciprocal on the SFU.
-__device__ __forceinline__ float2 gelu_as2(float2 x) {
-    const float2 z = __fmul2_rn(make_float2(fabsf(x.x), fabsf(x.y)), make_float2(0.70710678118654752f, 0.70710678118654752f));
-    // t = 1 / (1 + p z) on the SFU. (A cubic first guess plus two Newton steps on the FMA pipe, which
-    // frees the SFU, measured slower: 1159 against 1214 TFLOP/s on [189809 x 1024] x [1024 x 4096]; the
-    // epilogue is bound by instruction issue, not by the SFU.)
-    const float2 den = __ffma2_rn(make_float2(0.3275911f, 0.3275911f), z, make_float2(1.0f, 1.0f));
-    float2 t;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(den.x));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(den.y));
-    float2 p = __ffma2_rn(t, make_float2(0.5307027145f, 0.5307027145f), make_float2(-0.7265760135f, -0.7265760135f));
-    p = __ffma2_rn(t, p, make_float2(0.7107068705f, 0.7107068705f));
-    p = __ffma2_rn(t, p, make_float2(-0.142248368f, -0.142248368f));
-    p = __ffma2_rn(t, p, make_float2(0.127414796f, 0.127414796f));
-    p = __fmul2_rn(t, p);
-    // exp(-z^2) = 2^(-z^2 log2 e)
-    const float2 a = __fmul2_rn(__fmul2_rn(z, z), make_float2(-1.4426950408889634f, -1.4426950408889634f));
-    const float2 q = __fmul2_rn(p, make_float2(ex2f(a.x), ex2f(a.y)));
-    const float2 one_q = __fadd2_rn(make_float2(1.0f, 1.0f), make_float2(-q.x, -q.y));
-    return __fmul2_rn(x, make_float2(x.x >= 0.0f ? one_q.x : q.x, x.y >= 0.0f ? one_q.y : q.y));
-}
-
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(x), "r"(y), "r"(smem_u32(src))
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Byte offset of 16-byte chunk j of row r in a 32 x 64-byte sub-tile with the 64-byte swizzle of the
-// tensor map (chunk index XOR bits 1-2 of the row): conflict-free 16-byte accesses by 32 lanes.
-__device__ __forceinline__ int sw64(int r, int j) { return r * 64 + ((j ^ ((r >> 1) & 3)) << 4); }
 
 template <int BN, int STAGES, int EPI, bool PAIR, int LN>
 __global__ void __launch_bounds__(kThreads, 1)
