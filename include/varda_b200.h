@@ -281,6 +281,72 @@ int vb_layernorm(int dtype, const void* x, int64_t ldx, const float* w, const fl
 int vb_add_layernorm(int dtype, const void* a, const void* r, void* out1, const float* w, const float* b, void* ln,
                      int64_t ld, int64_t rows, int C, float eps, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit Linear layers, gated block norm
+ * No reference counterpart (the reference's types end at fp16). Matrices of microscaled 4-bit blocks (the
+ * OCP MXFP4 format): a row of K values in blocks of 32 columns, each with one scale byte s, 2^(s - 127)
+ * (255: the block is NaN), and 32 codes of the type e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives).
+ *   codes:  two per byte (even column in the low half), rows ldc bytes apart: 16-byte aligned, ldc a
+ *           multiple of 16, at least vb_mx4_row_bytes(K) = 16 ceil(K / 32); the last block's codes past K
+ *           are 0.
+ *   scales: vb_mx4_scale_bytes(rows, K) bytes, 16-byte aligned, in tiles of 128 rows x 4 blocks (512
+ *           bytes, block tiles of the same rows side by side): byte (row % 32) * 16 + (row % 128) / 32 * 4 +
+ *           block % 4 of tile (row / 128, block / 4). The bytes of a row's blocks past ceil(K / 32) must not
+ *           be 255 (the functions here write 0); those of rows past the last are not used.
+ * The same dtype, stream and error rules as above; nothing is allocated; calls may be captured. */
+int64_t vb_mx4_row_bytes(int64_t K);
+int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K);
+
+/* x [rows, K] of dtype -> 4-bit blocks: s = floor(log2 max|x|) - 2 + 127 (at least 0), code = x / scale to
+ * the nearest value, ties to the even code, magnitudes over 6 to 6; a block with Inf or NaN becomes NaN.
+ * Any ldx >= K; rows of 16-byte aligned starts are read fastest. Writes every scale byte of the tiles. */
+int vb_mx4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, void* codes, int64_t ldc,
+                    void* scales, void* stream);
+/* y [rows, K] of dtype = the values the blocks stand for (rounded to dtype: fp16 overflows to Inf). */
+int vb_mx4_dequantize(int dtype, const void* codes, int64_t ldc, const void* scales, int64_t rows, int64_t K, void* y,
+                      int64_t ldy, void* stream);
+
+/* vb_gemm on 4-bit blocks: Y[M, N] = A[M, K] W[N, K]^T (+ bias [N], may be NULL), then epilogue 0 = none, 1 =
+ * GELU (gelu_tanh selects the tanh form), 2 = + residual R[M, N]; bias, Y and R of dtype. Sums in fp32,
+ * rounded to dtype once, after the epilogue (vb_gemm rounds before its epilogue too). Y and R: 16-byte
+ * aligned, rows (ldy, ldr >= N elements) a multiple of 16 bytes apart; R may be Y. lda, ldw in bytes. */
+int vb_gemm_mx4(int dtype, const void* A, int64_t lda, const void* sA, const void* W, int64_t ldw, const void* sW,
+                const void* bias, void* Y, int64_t ldy, const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K,
+                int epilogue, int gelu_tanh, void* stream);
+
+/* The norms after and before a block, with its gate and the residual scale, in one pass:
+ *   x' = T(res_scale x + gate * post(h)),  y = T(pre(x') (1 + scale) + shift).
+ * post and pre: VB_NORM_NONE, VB_NORM_LAYER (mean and variance) or VB_NORM_RMS (mean square) over the C <= 16384
+ * columns, eps added to the variance, weight and bias fp32 [C] (either may be NULL). x, h, gate, scale,
+ * shift, out, y of dtype, leading dimensions in elements. h NULL: no block output (x' = T(res_scale x)).
+ * gate, scale, shift (each may be NULL): row r / rows_per_group of [groups, C] (rows_per_group 0: one row
+ * for all), scale and shift ldmod apart. out (x') may be NULL or x; y may be NULL, x or h (with that one's
+ * leading dimension, and not also out). y_codes with y_scales: y as 4-bit blocks instead (y must then be NULL;
+ * ldc in bytes; quantised from fp32, without the rounding to T). At least one output. */
+enum { VB_NORM_NONE = 0, VB_NORM_LAYER = 1, VB_NORM_RMS = 2 };
+typedef struct {
+    int64_t rows, C;
+    const void* x;
+    int64_t ldx;
+    const void* h;
+    int64_t ldh;
+    const float *post_w, *post_b;
+    const void* gate;
+    int64_t ldgate;
+    void* out;
+    int64_t ldo;
+    const float *pre_w, *pre_b;
+    const void *scale, *shift;
+    int64_t ldmod, rows_per_group;
+    void* y;
+    int64_t ldy;
+    void* y_codes;
+    int64_t ldc;
+    void* y_scales;
+    int post, pre;
+    float res_scale, eps;
+} vb_block_norm_args;
+int vb_block_norm(int dtype, const vb_block_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

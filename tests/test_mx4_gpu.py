@@ -1,0 +1,346 @@
+"""The 4-bit Linear layers and the gated block norm on the B200, against plain forms in 64 bits.
+
+Tolerances. Quantising and reading back are exact. A product's sum: at most K additions and a few operations
+of the epilogue, each off by at most one unit of the last place (2^-23) of the sum of magnitudes, then half a
+step of the type. A norm: a sum of C values is formed over at most 64 values per thread and 8 levels, so mean
+and variance are off by at most 80 2^-24 of the mean magnitude; with the few operations after it, 128 2^-24 =
+2^-17 of (|normalised value| + mean magnitude / spread + 1), then half a step of the type.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import mx4_reference as ref
+import varda_b200 as vb
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+HALF_STEP = {vb.FP16: 2.0 ** -11, vb.FP32: 2.0 ** -24}
+TINY = {vb.FP16: 2.0 ** -25, vb.FP32: 2.0 ** -149}  # half a step below the normal numbers
+
+
+def tdt(dt):
+    return torch.float16 if dt == vb.FP16 else torch.float32
+
+
+def put(a, dt, ld=None, pad=float("nan"), skew=0):
+    """Rows on the device, ld elements apart (NaN between them), `skew` elements past an aligned address."""
+    a = np.asarray(a)
+    rows, k = a.shape
+    ld = k if ld is None else ld
+    buf = torch.full((skew + rows * ld,), pad, device="cuda", dtype=tdt(dt))
+    v = buf[skew:].view(rows, ld)
+    v[:, :k] = torch.from_numpy(np.ascontiguousarray(a)).to("cuda", tdt(dt))
+    return v[:, :k]
+
+
+def get(t):
+    return t.detach().cpu().numpy()
+
+
+def rounded(a, dt):
+    return a.astype(np.float16 if dt == vb.FP16 else np.float32).astype(np.float64)
+
+
+def blocks(x):
+    """x in 64 bits -> (codes, tiles on the device, the values that they stand for)."""
+    c, s = ref.quantize(x)
+    return torch.from_numpy(c).cuda(), torch.from_numpy(ref.tile_scales(s)).cuda(), ref.values(c, s, x.shape[1])
+
+
+# ------------------------------------------------------------------ quantising
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 1024), (3, 31), (5, 32), (128, 33), (129, 127), (300, 129), (257, 1000),
+                                    (40, 4096)])
+def test_quantize_bits(rows, K, dt):
+    rng = np.random.default_rng(rows * 7 + K)
+    x = rounded(rng.normal(size=(rows, K)) * np.exp2(rng.integers(-20, 12, (rows, 1))), dt)
+    x[rng.random(x.shape) < 0.1] *= 0
+    x[0, 0] = -0.0
+    for ld, skew in ((K, 0), (K + 8 + (-K) % 8, 0), (K + 3, 1)):
+        d = put(x, dt, ld, skew=skew)
+        ldc = vb.mx4_row_bytes(K) + 16
+        codes = torch.full((rows + 1, ldc), 0xEE, device="cuda", dtype=torch.uint8)
+        tiles = torch.full((vb.mx4_scale_bytes(rows, K) + 16,), 0xEE, device="cuda", dtype=torch.uint8)
+        vb.mx4_quantize(dt, d, ld, rows, K, codes, ldc, tiles)
+        rc, rs = ref.quantize(x)
+        assert np.array_equal(get(codes)[:rows, :ldc - 16], rc)
+        assert (get(codes)[:, ldc - 16:] == 0xEE).all() and (get(codes)[rows] == 0xEE).all()
+        assert np.array_equal(get(tiles)[:-16], ref.tile_scales(rs)) and (get(tiles)[-16:] == 0xEE).all()
+        y = torch.full((rows + 1, ld), 7.0, device="cuda", dtype=tdt(dt))
+        vb.mx4_dequantize(dt, codes, ldc, tiles, rows, K, y, ld)
+        assert np.array_equal(get(y)[:rows, :K].astype(np.float64), rounded(ref.values(rc, rs, K), dt))
+        assert (get(y)[:, K:] == 7).all() and (get(y)[rows] == 7).all()
+
+
+def test_quantize_ties_ends_and_not_finite():
+    """Every tie and its neighbours, saturation, the ends of fp32, and blocks with Inf or NaN."""
+    grid = np.concatenate([ref.E2M1, (ref.E2M1[1:] + ref.E2M1[:-1]) / 2, [6.5, 7, 7.99]])
+    near = np.concatenate([grid, np.nextafter(grid.astype(np.float32), np.float32(9)), np.nextafter(grid.astype(np.float32), np.float32(0))])
+    rows = []
+    for e in (-126, -100, -1, 0, 5, 120, 125):
+        for part in np.array_split(near, 3):
+            r = np.zeros(32)
+            r[:len(part)] = part * (1 - 2 * (np.arange(len(part)) % 2))
+            r[31] = 4.0
+            rows.append(r * np.exp2(float(e)))
+    for lone in (2.0 ** -149, 2.0 ** -126, 2.0 ** -127, 3.4028234663852886e38, np.inf, -np.inf, np.nan):
+        r = np.linspace(-1, 1, 32) * 2.0 ** -130
+        r[5] = lone
+        rows.append(r)
+    x = np.array(rows, np.float32).astype(np.float64)
+    n = len(x)
+    codes, tiles = torch.zeros(n, 16, device="cuda", dtype=torch.uint8), torch.zeros(512, device="cuda", dtype=torch.uint8)
+    vb.mx4_quantize(vb.FP32, put(x, vb.FP32), 32, n, 32, codes, 16, tiles)
+    rc, rs = ref.quantize(x)
+    assert np.array_equal(ref.untile_scales(get(tiles), n, 1), rs) and (rs[-3:] == 255).all()
+    assert np.array_equal(get(codes), rc)
+    y = torch.zeros(n, 32, device="cuda")
+    vb.mx4_dequantize(vb.FP32, codes, 16, tiles, n, 32, y, 32)
+    np.testing.assert_array_equal(get(y), ref.values(rc, rs, 32).astype(np.float32))
+
+
+# ------------------------------------------------------------------ products
+
+def gelu(v, tanh=False):
+    if tanh:
+        return 0.5 * v * (1 + np.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
+    return 0.5 * v * np.array([math.erfc(-t * math.sqrt(0.5)) for t in v.ravel()]).reshape(v.shape)
+
+
+def product_case(M, N, K, dt, seed=0):
+    rng = np.random.default_rng(seed + M * 31 + N * 7 + K)
+    A = rng.normal(size=(M, K)) * np.exp(rng.normal(size=(M, 1)) + 0.5 * rng.normal(size=(1, K)))
+    W = rng.normal(size=(N, K)) / math.sqrt(K)
+    return blocks(A), blocks(W), rounded(rng.normal(size=N), dt), rounded(rng.normal(size=(M, N)), dt)
+
+
+def product_check(got, a, w, bias, R, dt, epi, tanh=False):
+    K = a.shape[1]
+    y, mag = a @ w.T, np.abs(a) @ np.abs(w).T
+    if bias is not None:
+        y, mag = y + bias, mag + np.abs(bias)
+    err = (K + 8) * 2.0 ** -23 * mag
+    if epi == 1:  # |gelu'| <= 1.13; its own operations (erf within 2^-22 of 1, a handful of roundings)
+        err = 1.13 * err + 2.0 ** -20 * np.abs(y)
+        y = gelu(y, tanh)
+    if epi == 2:
+        y, err = y + R, err + 2.0 ** -23 * (np.abs(y) + np.abs(R))
+    tol = err + HALF_STEP[dt] * (np.abs(y) + err) + TINY[dt]
+    bad = np.abs(got - y) > tol
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.max(np.abs(got - y) / tol):.2f} x the tolerance at {np.argwhere(bad)[0]}"
+
+
+def product_run(A, W, bias, R, M, N, K, dt, epi, tanh=False, ld=None):
+    ld = ld or (N + 7) // 8 * 8
+    y = torch.full((M + 1, ld), 7.0, device="cuda", dtype=tdt(dt))
+    r = put(R, dt, ld) if epi == 2 else None
+    b = None if bias is None else torch.from_numpy(bias).to("cuda", tdt(dt))
+    vb.gemm_mx4(dt, A[0], A[0].stride(0), A[1], W[0], W[0].stride(0), W[1], b, y, ld, r, ld, M, N, K, epi, tanh)
+    vb.check_device()
+    y = get(y).astype(np.float64)
+    assert (y[M] == 7).all() and (y[:, N:] == 7).all(), "wrote past the output"
+    return y[:M, :N]
+
+
+SHAPES = [(1, 1, 1), (1, 80, 32), (1, 4096, 1024), (2, 129, 33), (3, 1000, 200), (4, 31, 64), (5, 256, 1024), (8, 70, 2100),
+          (9, 1024, 4096), (17, 257, 96), (64, 512, 512), (127, 80, 184), (128, 128, 128), (129, 130, 160), (300, 1000, 1000),
+          (512, 300, 320), (1000, 2048, 512)]
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_product(M, N, K, dt):
+    A, W, bias, R = product_case(M, N, K, dt)
+    epi = (M + N + K) % 3
+    got = product_run(A, W, bias, R, M, N, K, dt, epi)
+    product_check(got, A[2], W[2], bias, R, dt, epi)
+
+
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("epi,tanh,has_bias", [(0, False, False), (0, False, True), (1, False, True), (1, True, True),
+                                               (2, False, False), (2, False, True)])
+def test_product_epilogues(M, epi, tanh, has_bias):
+    for dt in (vb.FP16, vb.FP32):
+        N, K = 200, 352
+        A, W, bias, R = product_case(M, N, K, dt, 3)
+        bias = bias if has_bias else None
+        got = product_run(A, W, bias, R, M, N, K, dt, epi, tanh, ld=208)
+        product_check(got, A[2], W[2], bias, R, dt, epi, tanh)
+
+
+@pytest.mark.parametrize("M", [2, 200])
+def test_product_nan_blocks_and_zero_rows(M):
+    """A NaN block makes its row (of A) or column (of W) NaN and nothing else; a row of zeros gives the bias."""
+    N, K = 96, 256
+    A, W, bias, R = product_case(M, N, K, vb.FP32, 5)
+    a, w = A[2].copy(), W[2].copy()
+    a[0] = 0
+    a[1, 100] = np.nan
+    w[7, 3] = np.inf
+    A, W = blocks(a), blocks(w)
+    got = product_run(A, W, bias, R, M, N, K, vb.FP32, 0)
+    nan = np.zeros((M, N), bool)
+    nan[1], nan[:, 7] = True, True
+    assert np.array_equal(np.isnan(got), nan)
+    keep = np.arange(N) != 7
+    assert np.array_equal(got[0, keep], bias[keep])
+
+
+@pytest.mark.parametrize("M", [2, 200])
+def test_product_residual_in_place_and_strided_codes(M):
+    """R is Y; codes whose rows are further apart than they need."""
+    N, K, dt = 136, 224, vb.FP16
+    A, W, bias, R = product_case(M, N, K, dt, 9)
+
+    def wide(c):
+        t = torch.full((c.shape[0], c.shape[1] + 48), 0xFF, device="cuda", dtype=torch.uint8)
+        t[:, :c.shape[1]] = c
+        return t
+
+    ca, cw, y = wide(A[0]), wide(W[0]), put(R, dt)
+    b = torch.from_numpy(bias).to("cuda", tdt(dt))
+    vb.gemm_mx4(dt, ca, ca.stride(0), A[1], cw, cw.stride(0), W[1], b, y, N, y, N, M, N, K, 2)
+    product_check(get(y).astype(np.float64), A[2], W[2], bias, R, dt, 2)
+
+
+# ------------------------------------------------------------------ block norm
+
+def norm_tol(v, n, size, w, b, dt):
+    """|normalised value| etc. -> tolerance of the norm's fp32 result."""
+    scale = 1.0 if w is None else np.abs(w)
+    return 2.0 ** -17 * (scale * (np.abs(n) + size + 1) + (0 if b is None else np.abs(b)))
+
+
+def norm_case(rows, C, dt, groups, rng, mean=0.0):
+    x, h = (rounded(rng.normal(size=(rows, C)) * s + mean, dt) for s in (2.0, 0.7))
+    g, sc, sh = (rounded(0.3 * rng.normal(size=(groups, C)), dt) for _ in range(3))
+    w = [(1 + 0.2 * rng.normal(size=C)).astype(np.float32) for _ in range(2)]
+    b = [(0.2 * rng.normal(size=C)).astype(np.float32) for _ in range(2)]
+    return x, h, g, sc, sh, w, b
+
+
+def norm_check(got_x, got_y, x, h, post, pw, pb, g, rs, pre, w, b, sc, sh, dt, eps=1e-5):
+    """x' against 64 bits; y against 64 bits of the norm of the x' that the kernel stored."""
+    t, e = rs * x, 2.0 ** -23 * np.abs(rs * x)
+    if h is not None:
+        n, size = ref.norm(h, post, None, None, eps)
+        p, _ = ref.norm(h, post, pw, pb, eps)
+        pe = norm_tol(h, n, size, pw, pb, dt) if post else 0
+        if g is not None:
+            p, pe = p * g, (pe + 2.0 ** -23 * np.abs(p)) * np.abs(g)
+        t, e = t + p, e + pe + 2.0 ** -23 * (np.abs(t) + np.abs(p))
+    tol = e + HALF_STEP[dt] * (np.abs(t) + e) + TINY[dt]
+    assert (np.abs(got_x - t) <= tol).all(), f"x': {np.max(np.abs(got_x - t) / tol):.2f} x the tolerance"
+    if got_y is None:
+        return
+    n, size = ref.norm(got_x, pre, None, None, eps)
+    y, _ = ref.norm(got_x, pre, w, b, eps)
+    e = norm_tol(got_x, n, size, w, b, dt) if pre else 0
+    if sc is not None:
+        y, e = y * (1 + sc), (e + 2.0 ** -22 * np.abs(y)) * (1 + np.abs(sc))
+    if sh is not None:
+        y, e = y + sh, e + 2.0 ** -23 * (np.abs(y) + np.abs(sh))
+    tol = e + HALF_STEP[dt] * (np.abs(y) + e) + TINY[dt]
+    assert (np.abs(got_y - y) <= tol).all(), f"y: {np.max(np.abs(got_y - y) / tol):.2f} x the tolerance"
+
+
+def norm_run(x, h, post, pw, pb, g, rs, pre, w, b, sc, sh, group, dt, ld=None, skew=0):
+    rows, C = x.shape
+    ld = ld or C
+    f32 = lambda a: None if a is None else torch.from_numpy(a).cuda()  # noqa: E731
+    opt = lambda a: None if a is None else put(a, dt, ld, skew=skew)  # noqa: E731
+    out, y = (torch.full((rows + 1, ld), 7.0, device="cuda", dtype=tdt(dt)) for _ in range(2))
+    vb.block_norm(dt, rows, C, put(x, dt, ld, skew=skew), ld, h=opt(h), ldh=ld, post=post, post_w=f32(pw), post_b=f32(pb),
+                  gate=opt(g), ldgate=ld, res_scale=rs, out=out, ldo=ld, pre=pre, pre_w=f32(w), pre_b=f32(b), scale=opt(sc),
+                  shift=opt(sh), ldmod=ld, rows_per_group=group, y=y, ldy=ld)
+    torch.cuda.synchronize()
+    for t in (out, y):
+        assert (t[rows] == 7).all() and (t[:, C:] == 7).all(), "wrote past the rows"
+    return get(out)[:rows, :C].astype(np.float64), get(y)[:rows, :C].astype(np.float64)
+
+
+NORM_SHAPES = [(1, 1), (2, 7), (9, 8), (5, 100), (3, 256), (1, 1024), (33, 1000), (7, 2048), (3, 2056), (2, 5000), (2, 16384),
+               (1300, 264), (1200, 1024), (1201, 2000), (1199, 517)]
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows,C", NORM_SHAPES)
+def test_block_norm(rows, C, dt):
+    rng = np.random.default_rng(rows + C)
+    i = rows + C
+    post, pre = i % 3, (i // 3) % 3
+    group = [0, 1, 2, max(1, rows // 3)][i % 4]
+    groups = -(-rows // group) if group else 1
+    at = np.arange(rows) // group if group else np.zeros(rows, int)
+    for ld, skew in ((C, 0), (C + 8 + (-C) % 8, 0), (C + 1, 1)):
+        x, h, g, sc, sh, w, b = norm_case(rows, C, dt, groups, rng, mean=[0, 5.0][rows % 2])
+        got = norm_run(x, h, post, w[0], b[0], g, 0.75, pre, w[1], b[1], sc, sh, group, dt, ld, skew)
+        norm_check(*got, x, h, post, w[0], b[0], g[at], 0.75, pre, w[1], b[1], sc[at], sh[at], dt)
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows", [3, 1500])
+def test_block_norm_without_parts(rows, dt):
+    """Each part absent; x' alone; in place."""
+    C = 384
+    rng = np.random.default_rng(rows)
+    x, h, g, sc, sh, w, b = norm_case(rows, C, dt, 1, rng)
+    at = np.zeros(rows, int)
+    for post in (0, 1, 2):
+        for pre in (0, 1, 2):
+            got = norm_run(x, None, post, w[0], b[0], g, 0.5, pre, None, b[1], sc, None, 0, dt)
+            norm_check(*got, x, None, post, None, None, None, 0.5, pre, None, b[1], sc[at], None, dt)
+            got = norm_run(x, h, post, None, None, None, 1.0, pre, w[1], None, None, sh, 0, dt)
+            norm_check(*got, x, h, post, None, None, None, 1.0, pre, w[1], None, None, sh[at], dt)
+    d, e, y = put(x, dt), put(h, dt), put(h, dt)
+    vb.block_norm(dt, rows, C, d, C, h=y, ldh=C, post=1, out=d, ldo=C, pre=1, y=y, ldy=C)  # x' over x, y over h
+    first = get(d).astype(np.float64), get(y).astype(np.float64)
+    norm_check(*first, x, h, 1, None, None, None, 1.0, 1, None, None, None, None, dt)
+    d = put(x, dt)
+    vb.block_norm(dt, rows, C, d, C, h=e, ldh=C, post=1, out=d, ldo=C)
+    assert np.array_equal(get(d).astype(np.float64), first[0])
+
+
+def test_block_norm_constant_rows_and_not_finite():
+    """A constant row normalises to zero (eps keeps it finite); NaN and Inf stay in their rows."""
+    C, dt = 512, vb.FP32
+    rng = np.random.default_rng(2)
+    x = rng.normal(size=(6, C))
+    x[1], x[2], x[3, 17], x[4, 3] = 0.0, 4.0, np.nan, np.inf
+    y = torch.zeros(6, C, device="cuda")
+    vb.block_norm(dt, 6, C, put(x, dt), C, pre=vb.NORM_LAYER, y=y, ldy=C)
+    got = get(y)
+    assert (got[1] == 0).all() and (got[2] == 0).all()
+    assert np.isnan(got[3]).all() and np.isnan(got[4]).any() and np.isfinite(got[[0, 5]]).all()
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows,C", [(1, 32), (3, 1000), (130, 96), (40, 1), (1300, 1024), (1250, 100), (5, 4100)])
+def test_block_norm_in_4_bits(rows, C, dt):
+    """The 4-bit output is the quantised fp32 y: with fp32 storage, the same bits as quantising the y it stores."""
+    rng = np.random.default_rng(rows + C)
+    x, h, g, sc, sh, w, b = norm_case(rows, C, dt, 1, rng)
+    f32 = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    kw = dict(h=put(h, dt), ldh=C, post=2, post_w=f32(w[0]), gate=put(g, dt), pre=1, pre_w=f32(w[1]), pre_b=f32(b[1]),
+              scale=put(sc, dt), shift=put(sh, dt))
+    y = torch.zeros(rows, C, device="cuda", dtype=tdt(dt))
+    vb.block_norm(dt, rows, C, put(x, dt), C, y=y, ldy=C, **kw)
+    nb, ldc = -(-C // 32), vb.mx4_row_bytes(C) + 16
+    codes = torch.full((rows + 1, ldc), 0xEE, device="cuda", dtype=torch.uint8)
+    tiles = torch.full((vb.mx4_scale_bytes(rows, C),), 0xEE, device="cuda", dtype=torch.uint8)
+    out = torch.zeros(rows, C, device="cuda", dtype=tdt(dt))
+    vb.block_norm(dt, rows, C, put(x, dt), C, y_codes=codes, ldc=ldc, y_scales=tiles, out=out, ldo=C, **kw)
+    assert (get(codes)[:, ldc - 16:] == 0xEE).all() and (get(codes)[rows] == 0xEE).all()
+    got_s = ref.untile_scales(get(tiles), rows, -(-nb // 4) * 4)
+    assert (got_s[:, nb:] == 0).all()
+    if dt == vb.FP32:
+        rc, rs = ref.quantize(get(y))
+        assert np.array_equal(got_s[:, :nb], rs) and np.array_equal(get(codes)[:rows, :ldc - 16], rc)
+    else:  # quantised before the rounding to fp16: within a code's step of y, half of it and y's own rounding
+        v = ref.values(get(codes)[:rows, :ldc - 16], got_s[:, :nb], C)
+        step = np.repeat(np.exp2(got_s[:, :nb].astype(np.float64) - 127), 32, 1)[:, :C] * 2.0
+        assert (np.abs(v - get(y)) <= step + 2.0 ** -10 * np.abs(get(y))).all()

@@ -11,14 +11,17 @@
 #include <memory>
 #include <string>
 
+#include "block_norm.cuh"
 #include "comm.h"
 #include "common.h"
 #include "config.h"
 #include "engine.h"
 #include "safetensors.h"
+#include "gemm_mx4.cuh"
 #include "gemm_tc.cuh"
 #include "graph.h"
 #include "kernels.cuh"
+#include "mx4.cuh"
 #include "shard.h"
 
 struct vb_model {
@@ -659,6 +662,135 @@ int vb_add_layernorm(int dtype, const void* a, const void* r, void* out1, const 
                                          static_cast<__half*>(out1), w, b, static_cast<__half*>(ln), ld, rows, C, eps,
                                          S(stream));
         else vb::fail(vb::kInvalidArgument, "dtype");
+    });
+}
+
+// ---------------------------------------------------------------- 4-bit Linear layers, gated block norm
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+void check(bool ok, const char* what) {
+    if (!ok) vb::fail(vb::kInvalidArgument, what);
+}
+
+int64_t dtype_size(int dtype) {
+    if (dtype == VB_PRECISION_FP32) return 4;
+    if (dtype == VB_PRECISION_FP16) return 2;
+    vb::fail(vb::kInvalidArgument, "dtype");
+}
+
+// sizes whose products stay far inside 64 bits, and row indices inside 32
+constexpr int64_t kMaxDim = INT32_MAX / 2;
+
+void check_blocks(const void* codes, int64_t ldc, const void* scales, int64_t K, const char* what) {
+    need(codes, what), need(scales, what);
+    if (!aligned16(codes) || ldc % 16 || ldc < vb::mx4::row_bytes(K) || !aligned16(scales))
+        vb::fail(vb::kInvalidArgument, std::string(what) + ": codes and scales must be 16-byte aligned, the codes' rows a "
+                                                           "multiple of 16 bytes that holds K");
+}
+
+}  // namespace
+
+int64_t vb_mx4_row_bytes(int64_t K) { return K > 0 ? vb::mx4::row_bytes(K) : 0; }
+int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K) { return rows > 0 && K > 0 ? vb::mx4::scale_bytes(rows, K) : 0; }
+
+int vb_mx4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, void* codes, int64_t ldc, void* scales,
+                    void* stream) {
+    return guard([&] {
+        dtype_size(dtype);
+        check(rows >= 0 && rows <= kMaxDim && K >= 1 && K <= kMaxDim, "mx4_quantize: rows, K");
+        if (rows == 0) return;
+        need(x, "x");
+        check(ldx >= K, "mx4_quantize: ldx");
+        check_blocks(codes, ldc, scales, K, "mx4_quantize");
+        auto* c = static_cast<uint8_t*>(codes);
+        auto* sc = static_cast<uint8_t*>(scales);
+        if (dtype == VB_PRECISION_FP32) vb::mx4::quantize(static_cast<const float*>(x), ldx, rows, K, c, ldc, sc, S(stream));
+        else vb::mx4::quantize(static_cast<const __half*>(x), ldx, rows, K, c, ldc, sc, S(stream));
+    });
+}
+
+int vb_mx4_dequantize(int dtype, const void* codes, int64_t ldc, const void* scales, int64_t rows, int64_t K, void* y,
+                      int64_t ldy, void* stream) {
+    return guard([&] {
+        dtype_size(dtype);
+        check(rows >= 0 && rows <= kMaxDim && K >= 1 && K <= kMaxDim, "mx4_dequantize: rows, K");
+        if (rows == 0) return;
+        need(y, "y");
+        check(ldy >= K, "mx4_dequantize: ldy");
+        check_blocks(codes, ldc, scales, K, "mx4_dequantize");
+        auto* c = static_cast<const uint8_t*>(codes);
+        auto* sc = static_cast<const uint8_t*>(scales);
+        if (dtype == VB_PRECISION_FP32) vb::mx4::dequantize(c, ldc, sc, rows, K, static_cast<float*>(y), ldy, S(stream));
+        else vb::mx4::dequantize(c, ldc, sc, rows, K, static_cast<__half*>(y), ldy, S(stream));
+    });
+}
+
+int vb_gemm_mx4(int dtype, const void* A, int64_t lda, const void* sA, const void* W, int64_t ldw, const void* sW,
+                const void* bias, void* Y, int64_t ldy, const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K,
+                int epilogue, int gelu_tanh, void* stream) {
+    return guard([&] {
+        const int64_t z = dtype_size(dtype);
+        check(epilogue >= 0 && epilogue <= 2, "epilogue");
+        check(M >= 0 && M <= kMaxDim && N >= 0 && N <= kMaxDim && K >= 1 && K <= kMaxDim, "gemm_mx4: M, N, K");
+        if (M == 0 || N == 0) return;
+        check_blocks(A, lda, sA, K, "gemm_mx4: A"), check_blocks(W, ldw, sW, K, "gemm_mx4: W");
+        need(Y, "Y");
+        check(aligned16(Y) && ldy >= N && ldy * z % 16 == 0, "gemm_mx4: Y must be 16-byte aligned, ldy >= N a multiple of 16 bytes");
+        if (epilogue == 2) {
+            need(R, "R");
+            check(aligned16(R) && ldr >= N && ldr * z % 16 == 0, "gemm_mx4: R must be 16-byte aligned, ldr >= N a multiple of 16 bytes");
+        }
+        auto run = [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            vb::mx4::GemmArgs<T> a;
+            a.A = static_cast<const uint8_t*>(A), a.lda = lda, a.sA = static_cast<const uint8_t*>(sA);
+            a.W = static_cast<const uint8_t*>(W), a.ldw = ldw, a.sW = static_cast<const uint8_t*>(sW);
+            a.bias = static_cast<const T*>(bias), a.Y = static_cast<T*>(Y), a.ldy = ldy;
+            a.R = static_cast<const T*>(R), a.ldr = ldr, a.M = M, a.N = N, a.K = K, a.epi = epilogue;
+            a.gelu_tanh = gelu_tanh != 0;
+            vb::mx4::gemm_rows(a, S(stream));
+        };
+        if (dtype == VB_PRECISION_FP32) run(static_cast<float*>(nullptr));
+        else run(static_cast<__half*>(nullptr));
+    });
+}
+
+int vb_block_norm(int dtype, const vb_block_norm_args* p, void* stream) {
+    return guard([&] {
+        dtype_size(dtype);
+        need(p, "args");
+        const vb_block_norm_args& q = *p;
+        auto kind = [](int n) { return n == VB_NORM_NONE || n == VB_NORM_LAYER || n == VB_NORM_RMS; };
+        check(kind(q.post) && kind(q.pre), "block_norm: post, pre");
+        check(q.rows >= 0 && q.rows <= kMaxDim && q.C >= 1 && q.rows_per_group >= 0, "block_norm: rows, C, rows_per_group");
+        if (q.C > vb::k::kBlockNormMaxC) vb::fail(vb::kUnsupported, "block_norm: C over 16384");
+        check(q.out || q.y || q.y_codes, "block_norm: no output");
+        check(!(q.y && q.y_codes), "block_norm: y and y_codes");
+        if (q.rows == 0) return;
+        need(q.x, "x");
+        check(q.ldx >= q.C && (!q.h || q.ldh >= q.C) && (!q.out || q.ldo >= q.C) && (!q.y || q.ldy >= q.C),
+              "block_norm: a leading dimension is less than C");
+        // one modulation row for all rows needs no leading dimension
+        const bool one = q.rows_per_group == 0 || q.rows_per_group >= q.rows;
+        check(one || ((!q.gate || q.ldgate >= q.C) && ((!q.scale && !q.shift) || q.ldmod >= q.C)), "block_norm: ldgate, ldmod");
+        if (q.y_codes) check_blocks(q.y_codes, q.ldc, q.y_scales, q.C, "block_norm: y_codes");
+        auto run = [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            vb::k::BlockNormArgs<T> a;
+            a.rows = q.rows, a.C = int(q.C), a.x = static_cast<const T*>(q.x), a.ldx = q.ldx;
+            a.h = static_cast<const T*>(q.h), a.ldh = q.ldh, a.post = q.post, a.post_w = q.post_w, a.post_b = q.post_b;
+            a.gate = static_cast<const T*>(q.gate), a.ldgate = one ? 0 : q.ldgate, a.res_scale = q.res_scale;
+            a.out = static_cast<T*>(q.out), a.ldo = q.ldo, a.pre = q.pre, a.pre_w = q.pre_w, a.pre_b = q.pre_b;
+            a.scale = static_cast<const T*>(q.scale), a.shift = static_cast<const T*>(q.shift);
+            a.ldmod = one ? 0 : q.ldmod, a.group = one ? 0 : q.rows_per_group;
+            a.y = static_cast<T*>(q.y), a.ldy = q.ldy, a.yc = static_cast<uint8_t*>(q.y_codes), a.ldyc = q.ldc;
+            a.ys = static_cast<uint8_t*>(q.y_scales), a.eps = q.eps;
+            vb::k::block_norm(a, S(stream));
+        };
+        if (dtype == VB_PRECISION_FP32) run(static_cast<float*>(nullptr));
+        else run(static_cast<__half*>(nullptr));
     });
 }
 

@@ -18,6 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvarda_b200.so")
 
 FP32, FP16 = 0, 1
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 ERRORS = {1: "invalid argument", 2: "format", 3: "cuda", 4: "unsupported", 5: "internal", 6: "timeout"}
 
 
@@ -73,6 +74,12 @@ def _load_lib():
         "vb_fold_layernorm": ([P, I64, I64, I, P, P, P, P, P], I),
         "vb_row_seg_stats": ([P, I64, I64, I, I, P, P], I),
         "vb_add_layernorm": ([I, P, P, P, P, P, P, I64, I64, I, F, P], I),
+        "vb_mx4_row_bytes": ([I64], I64),
+        "vb_mx4_scale_bytes": ([I64, I64], I64),
+        "vb_mx4_quantize": ([I, P, I64, I64, I64, P, I64, P, P], I),
+        "vb_mx4_dequantize": ([I, P, I64, P, I64, I64, P, I64, P], I),
+        "vb_gemm_mx4": ([I, P, I64, P, P, I64, P, P, P, I64, P, I64, I64, I64, I64, I, I, P], I),
+        "vb_block_norm": ([I, P, P], I),
         "vb_rollout": ([P, P, I, P, P, I, P, P, P], I),
         "vb_attention_rows": ([I, P, P, P, I64, P, I64, P, P, I64, P, I64, P, I64, P, I, I, I, P], I),
         "vb_attention_split_noalloc": ([I, P, P, I64, I64, P, I64, P, P, I64, P, I64, P, I64, P, I, I, I, I, P], I),
@@ -401,6 +408,54 @@ def layernorm(dtype, x, ldx, w, b, y, ldy, rows, C, eps, stream=None):
 def add_layernorm(dtype, a, r, out1, w, b, ln, ld, rows, C, eps, stream=None):
     check(lib.vb_add_layernorm(dtype, _ptr(a), _ptr(r), _ptr(out1), _ptr(w), _ptr(b), _ptr(ln), ld, rows, C, eps,
                                stream))
+
+
+def mx4_row_bytes(K):
+    """Bytes of a row of K 4-bit codes (the least ldc)."""
+    return lib.vb_mx4_row_bytes(K)
+
+
+def mx4_scale_bytes(rows, K):
+    """Bytes of the scale tiles of a [rows, K] matrix of 4-bit blocks."""
+    return lib.vb_mx4_scale_bytes(rows, K)
+
+
+def mx4_quantize(dtype, x, ldx, rows, K, codes, ldc, scales, stream=None):
+    check(lib.vb_mx4_quantize(dtype, _ptr(x), ldx, rows, K, _ptr(codes), ldc, _ptr(scales), stream))
+
+
+def mx4_dequantize(dtype, codes, ldc, scales, rows, K, y, ldy, stream=None):
+    check(lib.vb_mx4_dequantize(dtype, _ptr(codes), ldc, _ptr(scales), rows, K, _ptr(y), ldy, stream))
+
+
+def gemm_mx4(dtype, A, lda, sA, W, ldw, sW, bias, Y, ldy, R, ldr, M, N, K, epilogue=0, gelu_tanh=False, stream=None):
+    """vb_gemm_mx4: the product of two matrices of 4-bit blocks (codes and scale tiles each)."""
+    check(lib.vb_gemm_mx4(dtype, _ptr(A), lda, _ptr(sA), _ptr(W), ldw, _ptr(sW), _ptr(bias), _ptr(Y), ldy, _ptr(R), ldr,
+                          M, N, K, epilogue, int(gelu_tanh), stream))
+
+
+class BlockNormArgs(ctypes.Structure):
+    """vb_block_norm_args."""
+    _fields_ = [("rows", ctypes.c_int64), ("C", ctypes.c_int64), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+                ("h", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("post_w", ctypes.c_void_p),
+                ("post_b", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("ldgate", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("pre_w", ctypes.c_void_p),
+                ("pre_b", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+                ("ldmod", ctypes.c_int64), ("rows_per_group", ctypes.c_int64), ("y", ctypes.c_void_p),
+                ("ldy", ctypes.c_int64), ("y_codes", ctypes.c_void_p), ("ldc", ctypes.c_int64),
+                ("y_scales", ctypes.c_void_p), ("post", ctypes.c_int), ("pre", ctypes.c_int),
+                ("res_scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+def block_norm(dtype, rows, C, x, ldx, h=None, ldh=0, post=NORM_NONE, post_w=None, post_b=None, gate=None, ldgate=0,
+               res_scale=1.0, out=None, ldo=0, pre=NORM_NONE, pre_w=None, pre_b=None, scale=None, shift=None, ldmod=0,
+               rows_per_group=0, y=None, ldy=0, y_codes=None, ldc=0, y_scales=None, eps=1e-5, stream=None):
+    """vb_block_norm: x' = res_scale x + gate * post(h) to `out`, pre(x') (1 + scale) + shift to `y` or, as 4-bit
+    blocks, to `y_codes` and `y_scales`."""
+    a = BlockNormArgs(rows, C, _ptr(x), ldx, _ptr(h), ldh, _ptr(post_w), _ptr(post_b), _ptr(gate), ldgate, _ptr(out), ldo,
+                      _ptr(pre_w), _ptr(pre_b), _ptr(scale), _ptr(shift), ldmod, rows_per_group, _ptr(y), ldy,
+                      _ptr(y_codes), ldc, _ptr(y_scales), post, pre, res_scale, eps)
+    check(lib.vb_block_norm(dtype, ctypes.byref(a), stream))
 
 
 def rollout_update(window, T, rows, V_in, y_own, y_halo, n_own, V_out, f, F, kind, src, stream=None):
