@@ -313,6 +313,12 @@ int vb_gemm_mx4(int dtype, const void* A, int64_t lda, const void* sA, const voi
                 const void* bias, void* Y, int64_t ldy, const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K,
                 int epilogue, int gelu_tanh, void* stream);
 
+/* The same with the output as 4-bit blocks (codes, ldc in bytes; scales): the fp32 result of epilogue 0 or 1
+ * quantised as by vb_mx4_quantize; bias of dtype. The next product's A without a pass in between. */
+int vb_gemm_mx4_quant(int dtype, const void* A, int64_t lda, const void* sA, const void* W, int64_t ldw, const void* sW,
+                      const void* bias, void* codes, int64_t ldc, void* scales, int64_t M, int64_t N, int64_t K,
+                      int epilogue, int gelu_tanh, void* stream);
+
 /* The norms after and before a block, with its gate and the residual scale, in one pass:
  *   x' = T(res_scale x + gate * post(h)),  y = T(pre(x') (1 + scale) + shift).
  * post and pre: VB_NORM_NONE, VB_NORM_LAYER (mean and variance) or VB_NORM_RMS (mean square) over the C <= 16384

@@ -30,6 +30,17 @@ def quantize(x):
     return code[..., 0] | (code[..., 1] << 4), sb
 
 
+def round_to(x, sb):
+    """x [rows, K] in 64 bits rounded to the values of blocks with the scale bytes sb [rows, nb]."""
+    f = np.repeat(np.exp2(sb.astype(np.float64) - 127), 32, 1)[:, :x.shape[1]]
+    a = np.abs(x) / f
+    code = np.zeros(a.shape, int)
+    for i in range(7):
+        mid = (E2M1[i] + E2M1[i + 1]) / 2
+        code += (a >= mid) if i % 2 else (a > mid)
+    return np.copysign(E2M1[code] * f, x)
+
+
 def values(codes, sb, k):
     """The values [rows, k] in 64 bits."""
     c = np.stack((codes & 15, codes >> 4), -1).reshape(codes.shape[0], -1)

@@ -63,6 +63,14 @@ def test_gemm_refuses(bad):
     refused(lambda: vb.gemm_mx4(**{**GEMM, **bad}))
 
 
+@pytest.mark.parametrize("bad", [dict(dtype=7), dict(A=None), dict(lda=16), dict(sA=P + 2), dict(W=P + 4), dict(ldw=0),
+                                 dict(sW=None), dict(codes=None), dict(codes=P + 8), dict(ldc=32), dict(ldc=56),
+                                 dict(scales=None), dict(scales=P + 8), dict(M=-1), dict(N=-1), dict(K=0), dict(epilogue=2)])
+def test_gemm_quant_refuses(bad):
+    good = dict(dtype=vb.FP16, A=P, lda=32, sA=P, W=P, ldw=32, sW=P, bias=P, codes=P, ldc=48, scales=P, M=5, N=70, K=64, epilogue=1)
+    refused(lambda: vb.gemm_mx4_quant(**{**good, **bad}))
+
+
 NORM = dict(dtype=vb.FP16, rows=4, C=64, x=P, ldx=64, h=P, ldh=64, post=1, gate=P, ldgate=64, out=P, ldo=64, pre=2,
             scale=P, shift=P, ldmod=64, rows_per_group=2, y=P, ldy=64)
 

@@ -108,7 +108,7 @@ def test_quantize_ties_ends_and_not_finite():
 def gelu(v, tanh=False):
     if tanh:
         return 0.5 * v * (1 + np.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
-    return 0.5 * v * np.array([math.erfc(-t * math.sqrt(0.5)) for t in v.ravel()]).reshape(v.shape)
+    return 0.5 * v * torch.special.erfc(torch.from_numpy(-v * math.sqrt(0.5)).cuda()).cpu().numpy()
 
 
 def product_case(M, N, K, dt, seed=0):
@@ -118,7 +118,8 @@ def product_case(M, N, K, dt, seed=0):
     return blocks(A), blocks(W), rounded(rng.normal(size=N), dt), rounded(rng.normal(size=(M, N)), dt)
 
 
-def product_check(got, a, w, bias, R, dt, epi, tanh=False):
+def product_exact(a, w, bias, R, epi, tanh):
+    """(the result in 64 bits, the bound of an fp32 evaluation's error)."""
     K = a.shape[1]
     y, mag = a @ w.T, np.abs(a) @ np.abs(w).T
     if bias is not None:
@@ -129,6 +130,11 @@ def product_check(got, a, w, bias, R, dt, epi, tanh=False):
         y = gelu(y, tanh)
     if epi == 2:
         y, err = y + R, err + 2.0 ** -23 * (np.abs(y) + np.abs(R))
+    return y, err
+
+
+def product_check(got, a, w, bias, R, dt, epi, tanh=False):
+    y, err = product_exact(a, w, bias, R, epi, tanh)
     tol = err + HALF_STEP[dt] * (np.abs(y) + err) + TINY[dt]
     bad = np.abs(got - y) > tol
     assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.max(np.abs(got - y) / tol):.2f} x the tolerance at {np.argwhere(bad)[0]}"
@@ -148,7 +154,8 @@ def product_run(A, W, bias, R, M, N, K, dt, epi, tanh=False, ld=None):
 
 SHAPES = [(1, 1, 1), (1, 80, 32), (1, 4096, 1024), (2, 129, 33), (3, 1000, 200), (4, 31, 64), (5, 256, 1024), (8, 70, 2100),
           (9, 1024, 4096), (17, 257, 96), (64, 512, 512), (127, 80, 184), (128, 128, 128), (129, 130, 160), (300, 1000, 1000),
-          (512, 300, 320), (1000, 2048, 512)]
+          (512, 300, 320), (1000, 2048, 512), (2400, 1024, 544), (4600, 1024, 96), (5000, 1024, 1000), (20000, 800, 320),
+          (40000, 80, 256)]
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
@@ -205,6 +212,31 @@ def test_product_residual_in_place_and_strided_codes(M):
     b = torch.from_numpy(bias).to("cuda", tdt(dt))
     vb.gemm_mx4(dt, ca, ca.stride(0), A[1], cw, cw.stride(0), W[1], b, y, N, y, N, M, N, K, 2)
     product_check(get(y).astype(np.float64), A[2], W[2], bias, R, dt, 2)
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 64, 64), (3, 70, 200), (7, 192, 96), (129, 100, 64), (300, 1000, 320),
+                                   (2400, 1000, 224), (5000, 1024, 96), (20000, 800, 160)])
+def test_product_in_4_bits(M, N, K, dt):
+    """The output blocks: scale and values are those of some number within the fp32 error of the exact one."""
+    A, W, bias, _ = product_case(M, N, K, dt, 1)
+    epi = (M + N) % 2
+    nb, ldc = -(-N // 32), vb.mx4_row_bytes(N) + 16
+    codes = torch.full((M + 1, ldc), 0xEE, device="cuda", dtype=torch.uint8)
+    tiles = torch.full((vb.mx4_scale_bytes(M, N),), 0xEE, device="cuda", dtype=torch.uint8)
+    b = torch.from_numpy(bias).to("cuda", tdt(dt))
+    vb.gemm_mx4_quant(dt, A[0], A[0].stride(0), A[1], W[0], W[0].stride(0), W[1], b, codes, ldc, tiles, M, N, K, epi)
+    vb.check_device()
+    c = get(codes)
+    assert (c[:, ldc - 16:] == 0xEE).all() and (c[M] == 0xEE).all()
+    sb = ref.untile_scales(get(tiles), M, -(-nb // 4) * 4)
+    assert (sb[:, nb:] == 0).all()
+    y, err = product_exact(A[2], W[2], bias, None, epi, False)
+    low, high = np.maximum(np.abs(y) - err, 0), np.abs(y) + err
+    assert (ref.quantize(low)[1] <= sb[:, :nb]).all() and (sb[:, :nb] <= ref.quantize(high)[1]).all()
+    v = ref.values(c[:M, :ldc - 16], sb[:, :nb], 32 * nb)
+    assert (v[:, N:] == 0).all()
+    assert (ref.round_to(y - err, sb[:, :nb]) <= v[:, :N]).all() and (v[:, :N] <= ref.round_to(y + err, sb[:, :nb])).all()
 
 
 # ------------------------------------------------------------------ block norm

@@ -73,6 +73,7 @@ void need(const void* p, const char* what) {
 // The kernels' device-side timeout flags (read and cleared; synchronises the device).
 void device_errors() {
     if (vb::tc::take_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the tensor-core GEMM");
+    if (vb::mx4::take_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the 4-bit GEMM");
     if (vb::k::take_attention_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the attention");
 }
 
@@ -750,7 +751,32 @@ int vb_gemm_mx4(int dtype, const void* A, int64_t lda, const void* sA, const voi
             a.bias = static_cast<const T*>(bias), a.Y = static_cast<T*>(Y), a.ldy = ldy;
             a.R = static_cast<const T*>(R), a.ldr = ldr, a.M = M, a.N = N, a.K = K, a.epi = epilogue;
             a.gelu_tanh = gelu_tanh != 0;
-            vb::mx4::gemm_rows(a, S(stream));
+            vb::mx4::gemm(a, S(stream));
+        };
+        if (dtype == VB_PRECISION_FP32) run(static_cast<float*>(nullptr));
+        else run(static_cast<__half*>(nullptr));
+    });
+}
+
+int vb_gemm_mx4_quant(int dtype, const void* A, int64_t lda, const void* sA, const void* W, int64_t ldw, const void* sW,
+                      const void* bias, void* codes, int64_t ldc, void* scales, int64_t M, int64_t N, int64_t K,
+                      int epilogue, int gelu_tanh, void* stream) {
+    return guard([&] {
+        dtype_size(dtype);
+        check(epilogue == 0 || epilogue == 1, "gemm_mx4_quant: epilogue must be 0 or 1");
+        check(M >= 0 && M <= kMaxDim && N >= 0 && N <= kMaxDim && K >= 1 && K <= kMaxDim, "gemm_mx4_quant: M, N, K");
+        if (M == 0 || N == 0) return;
+        check_blocks(A, lda, sA, K, "gemm_mx4_quant: A"), check_blocks(W, ldw, sW, K, "gemm_mx4_quant: W");
+        check_blocks(codes, ldc, scales, N, "gemm_mx4_quant: codes");
+        auto run = [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            vb::mx4::GemmArgs<T> a;
+            a.A = static_cast<const uint8_t*>(A), a.lda = lda, a.sA = static_cast<const uint8_t*>(sA);
+            a.W = static_cast<const uint8_t*>(W), a.ldw = ldw, a.sW = static_cast<const uint8_t*>(sW);
+            a.bias = static_cast<const T*>(bias), a.Yc = static_cast<uint8_t*>(codes), a.ldyc = ldc;
+            a.Ys = static_cast<uint8_t*>(scales), a.M = M, a.N = N, a.K = K, a.epi = epilogue;
+            a.gelu_tanh = gelu_tanh != 0;
+            vb::mx4::gemm(a, S(stream));
         };
         if (dtype == VB_PRECISION_FP32) run(static_cast<float*>(nullptr));
         else run(static_cast<__half*>(nullptr));

@@ -34,5 +34,10 @@ template <class T> struct GemmArgs {
 
 // Few rows of A, on the CUDA cores (Y only). Enqueues on s: no allocation, no synchronisation.
 template <class T> void gemm_rows(const GemmArgs<T>& a, cudaStream_t s);
+// Any number of rows, Y or 4-bit output: on the tensor cores, or gemm_rows. Y and R 16-byte aligned, their rows
+// a multiple of 16 bytes apart. Enqueues on s: no allocation, no synchronisation.
+template <class T> void gemm(const GemmArgs<T>& a, cudaStream_t s);
+// Reads and clears the device-side error flag of the bounded waits (synchronises); 0: none timed out.
+int take_error();
 
 }  // namespace vb::mx4

@@ -573,16 +573,10 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 // box [box_rows, box_cols], zero fill out of bounds (loads) / clipped (stores).
 CUtensorMap make_map(const __half* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols = BK,
                      CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
-    CUtensorMap m;
     const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
     const cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
     const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, strides,
-                                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) fail(kCuda, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
-    return m;
+    return tensor_map(base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, dims, strides, box, swz);
 }
 
 // Per-stream tile counters for the dynamic tile order of launches that bring no counter of their own
@@ -735,6 +729,17 @@ int take_error() {
     VB_CUDA(cudaMemcpyFromSymbol(&e, g_error, sizeof(int)));
     if (e) VB_CUDA(cudaMemcpyToSymbol(g_error, &zero, sizeof(int)));
     return e;
+}
+
+CUtensorMap tensor_map(const void* base, CUtensorMapDataType type, int rank, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz) {
+    CUtensorMap m;
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode_fn()(&m, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, estr,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail(kCuda, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return m;
 }
 
 CUtensorMap tensor_map_2d(const __half* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols,

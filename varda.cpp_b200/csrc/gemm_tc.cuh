@@ -29,6 +29,10 @@ void gemm(const k::GemmArgs<__half>& a, cudaStream_t s, unsigned* sched);
 // (synchronises the device). Returns 0 when no wait timed out.
 int take_error();
 
+// Tensor map of rank 2 or 3 (dims and box innermost first, strides in bytes from the second dimension on):
+// out-of-bounds loads read zeros, stores are clipped.
+CUtensorMap tensor_map(const void* base, CUtensorMapDataType type, int rank, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz);
 // 2-D fp16 tensor map over a row-major [rows, cols] matrix with leading dimension ld (elements):
 // box [box_rows, box_cols] with the given shared-memory swizzle; out-of-bounds loads read zeros.
 CUtensorMap tensor_map_2d(const __half* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols,

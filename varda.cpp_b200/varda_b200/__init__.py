@@ -79,6 +79,7 @@ def _load_lib():
         "vb_mx4_quantize": ([I, P, I64, I64, I64, P, I64, P, P], I),
         "vb_mx4_dequantize": ([I, P, I64, P, I64, I64, P, I64, P], I),
         "vb_gemm_mx4": ([I, P, I64, P, P, I64, P, P, P, I64, P, I64, I64, I64, I64, I, I, P], I),
+        "vb_gemm_mx4_quant": ([I, P, I64, P, P, I64, P, P, P, I64, P, I64, I64, I64, I, I, P], I),
         "vb_block_norm": ([I, P, P], I),
         "vb_rollout": ([P, P, I, P, P, I, P, P, P], I),
         "vb_attention_rows": ([I, P, P, P, I64, P, I64, P, P, I64, P, I64, P, I64, P, I, I, I, P], I),
@@ -432,6 +433,13 @@ def gemm_mx4(dtype, A, lda, sA, W, ldw, sW, bias, Y, ldy, R, ldr, M, N, K, epilo
     """vb_gemm_mx4: the product of two matrices of 4-bit blocks (codes and scale tiles each)."""
     check(lib.vb_gemm_mx4(dtype, _ptr(A), lda, _ptr(sA), _ptr(W), ldw, _ptr(sW), _ptr(bias), _ptr(Y), ldy, _ptr(R), ldr,
                           M, N, K, epilogue, int(gelu_tanh), stream))
+
+
+def gemm_mx4_quant(dtype, A, lda, sA, W, ldw, sW, bias, codes, ldc, scales, M, N, K, epilogue=0, gelu_tanh=False,
+                   stream=None):
+    """vb_gemm_mx4_quant: the same with the output as 4-bit blocks (epilogue 0 or 1)."""
+    check(lib.vb_gemm_mx4_quant(dtype, _ptr(A), lda, _ptr(sA), _ptr(W), ldw, _ptr(sW), _ptr(bias), _ptr(codes), ldc,
+                                _ptr(scales), M, N, K, epilogue, int(gelu_tanh), stream))
 
 
 class BlockNormArgs(ctypes.Structure):
