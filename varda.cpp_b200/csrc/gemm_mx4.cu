@@ -1,21 +1,24 @@
 // The 4-bit product on the tensor cores (see gemm_mx4.cuh): tcgen05.mma kind::mxf4 with block scales, which
 // multiplies 64 e2m1 values of a row and column at a time, each block of 32 with its two scales, into fp32.
 //
-// Persistent and warp-specialised as the fp16 GEMM (gemm_tc.cu): one 320-thread CTA per SM, or clusters of
-// two with cta_group::2 computing 256-row tiles together.
-//   warp 0 (one lane)   TMA producer, per 256 columns of K: codes of A [128 x 128 bytes] and of W, 128-byte
-//                       swizzle, and their scale tiles (512 bytes per 128 rows and 128 columns, stored in
-//                       the order tcgen05.cp takes), into a ring of STAGES.
-//   warp 1 (one lane)   MMA issuer: tcgen05.cp of the stage's scales into one of two tensor-memory buffers
-//                       (every lane quarter gets a copy), then 4 MMAs of K = 64; in a last stage that K
-//                       cuts, only those it needs. A buffer is overwritten once the MMAs of two stages ago
-//                       have completed.
-//   warps 2-9           epilogue: 32 columns at a time from tensor memory, bias / GELU / residual in fp32, one
-//                       rounding, and a TMA store from swizzled shared memory; or 4-bit output: a lane holds
-//                       one row's block of 32 columns, so its scale is the maximum of the lane's registers.
-// Tensor memory at BN = 256: two accumulators would fill all 512 columns, but the scales need 48. So the
-// second starts at column 192, over the last 64 columns of the first, and both epilogues read those shared
-// columns first: the next tile's MMAs start when they have been read, a quarter into the epilogue.
+// Persistent and warp-specialised: one 768-thread CTA per SM, or clusters of two with cta_group::2 computing
+// 256-row tiles together (each CTA loads its 128 rows of A and half of the W tile).
+//   warp 0 (one lane)   TMA producer: codes of A [128 x 128 bytes = 256 columns of K] and of W, 128-byte
+//                       swizzle, into a ring of kStages.
+//   warp 2 (one lane)   TMA producer of their scale tiles (512 bytes per 128 rows and 128 columns, stored in
+//                       the order in which tensor memory holds them) into a ring of kSlots.
+//   warps 4-7           scales from shared into tensor memory, each warp its lane quarter's copy, into the buffer
+//                       of the stage (as many as stages). (tcgen05.cp does the same from the MMA thread, but
+//                       the tensor pipe runs it between the MMAs: 57 cycles per 512 bytes, 2970 TFLOP/s at most.)
+//   warp 1 (one lane)   MMA issuer: four MMAs of K = 64 per stage; in a last stage that K cuts, only those it needs.
+//   warps 8-23          epilogue: a warp takes 32 rows and a quarter of the tile's columns into registers at
+//                       once and hands the accumulator back, then bias / GELU / residual in fp32, one rounding
+//                       and a TMA store from swizzled shared memory (the residual came by TMA into the same
+//                       buffer meanwhile); or 4-bit output: a lane holds whole blocks of its row, so a
+//                       block's scale is the maximum of the lane's registers.
+// Tensor memory at BN = 256: two accumulators would fill all 512 columns, but the scales need some. So the
+// second accumulator starts at column 128, over half of the first; since the epilogue reads all columns
+// at once, the next tile's MMAs start a few hundred cycles after the last one's.
 //
 // Every wait is bounded as in gemm_tc.cu: on timeout a CTA sets the device error flag, stops issuing, waits for
 // its own copies and MMAs in flight, frees its tensor memory and returns.
@@ -40,7 +43,10 @@ using namespace vb::d;
 using namespace vb::ptx;
 
 constexpr int BM = 128, BKB = 128;  // rows of a CTA's tile; bytes of codes per row and stage (256 columns)
-constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
+constexpr int kEpiWarps = 16, kEpiWarp0 = 8, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+// registers: the first two warpgroups give back to the epilogue's four (2 x 40 + 4 x 96 <= 6 x the 80 of the launch)
+constexpr int kLaunchRegs = 80, kFewRegs = 40, kEpiRegs = 96;
+static_assert(2 * kFewRegs + 4 * kEpiRegs <= 6 * kLaunchRegs, "register split over what the CTA is launched with");
 constexpr unsigned long long kTimeoutNs = 4000000000ull;  // 4 s
 
 __device__ int g_error = 0;
@@ -57,6 +63,7 @@ struct Params {
     int64_t ktiles_out;
     int M, N, K64;  // K64: MMAs along K, ceil(K / 64)
     int gelu_tanh;
+    int bias16;  // bias is 16-byte aligned
 };
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
@@ -82,49 +89,52 @@ __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
         }
 }
 
-template <bool PAIR>
-__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-    if (PAIR) tma_load_2d_pair(dst, map, bar, x, y);
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                smem_u32(dst)),
-            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-            : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-    if (PAIR)
-        asm volatile(
-            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-            "%4}], [%5];" ::"r"(smem_u32(dst)),
-            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-            : "memory");
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-            "[%5];" ::"r"(smem_u32(dst)),
-            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-            : "memory");
+// After an abort: time for the loads already issued to land before the CTA exits (their barriers may also wait
+// for arrivals that will not come, or belong to the pair's other CTA).
+__device__ __forceinline__ void settle() {
+    const uint64_t t0 = now_ns();
+    while (now_ns() - t0 < 2000000ull) {
+    }
 }
 
-// Shared-memory descriptors. Codes: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart. Scales: 32
-// rows of 16 bytes without swizzle, 8-row groups 128 bytes apart.
+template <bool PAIR>
+__device__ __forceinline__ void load_codes(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+    if (PAIR) tma_load_2d_pair(dst, map, mapa(smem_u32(bar), 0), x, y);  // completes on the leader's barrier
+    else tma_load_2d(dst, map, bar, x, y);
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Arrival on a barrier of the pair that tells of tensor memory read or written: tcgen05.fence orders that, and
+// no other memory goes with it. (A release at cluster scope waits about 1000 cycles for the thread's other
+// writes: 1000 us instead of 330 on [189809 x 4096] x [4096 x 1024].)
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Shared-memory descriptor of the codes: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t codes_desc(uint32_t saddr) {
     return uint64_t((saddr & 0x3FFFF) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
-}
-__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) {
-    return uint64_t((saddr & 0x3FFFF) >> 4) | uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
 }
 // Instruction descriptor of kind::mxf4: A = B = e2m1 (1), scales ue8m0, K-major, K = 64; sf: which two of a
 // 32-bit column's four scale bytes (0 or 2).
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, int sf) {
     return uint32_t(sf) << 4 | 1u << 7 | 1u << 10 | uint32_t(n >> 3) << 17 | 1u << 23 | uint32_t(m >> 7) << 27 | uint32_t(sf) << 29;
 }
-template <bool PAIR> __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+// Scales into tensor memory: this lane's 16 bytes of a tile (rows lane + 32 i in column i) at column taddr.
+__device__ __forceinline__ void st_scales(uint32_t taddr, uint4 v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
 }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 template <bool PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                     uint32_t acc) {
@@ -140,60 +150,91 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
             "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
 }
 
+// GELU in fp32 with one special-function operation: x Phi(x) = max(x, 0) - z Phi(-z), z = |x|, and
+// Phi(-z) = 2^P(z) with P a polynomial fitted to log2 Phi(-z) on [0, 5.6] (weighted least squares towards the
+// smallest largest error of z Phi(-z)): |error| <= 3e-7, at most 5e-7 |x|. Past 5.6, z Phi(-z) stays at its
+// 6e-8. (The two-operation form of gemm_tc.cu is bound by the special-function units here: 16 a clock and
+// SM make 345 us on [189809 x 1024] x [1024 x 4096].)
+__device__ __forceinline__ float2 gelu2(float2 x) {
+    const float2 n = make_float2(fmaxf(-fabsf(x.x), -5.6f), fmaxf(-fabsf(x.y), -5.6f));
+    float2 p = __ffma2_rn(n, make_float2(3.26786503e-05f, 3.26786503e-05f), make_float2(7.58978247e-04f, 7.58978247e-04f));
+    p = __ffma2_rn(n, p, make_float2(8.02492630e-03f, 8.02492630e-03f));
+    p = __ffma2_rn(n, p, make_float2(5.32902256e-02f, 5.32902256e-02f));
+    p = __ffma2_rn(n, p, make_float2(-4.58889902e-01f, -4.58889902e-01f));
+    p = __ffma2_rn(n, p, make_float2(1.15115345f, 1.15115345f));
+    p = __ffma2_rn(n, p, make_float2(-9.99998868e-01f, -9.99998868e-01f));
+    float2 r;  // max(x, 0), NaN kept
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.x) : "f"(x.x));
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.y) : "f"(x.y));
+    return __ffma2_rn(n, make_float2(ex2f(p.x), ex2f(p.y)), r);
+}
+
 // T: type of bias, residual and output. OUT4: 4-bit output (T is the bias's type).
 template <class T, int BN, bool PAIR, bool OUT4> struct Layout {
     static constexpr int kNTiles = BN > 128 ? BN / 128 : 1;  // scale tiles of W per 128 columns of K
     static constexpr int kA = BM * BKB, kB = (PAIR ? BN / 2 : BN) * BKB;
     static constexpr int kSA = 2 * 512, kSB = 2 * 512 * kNTiles;
-    static constexpr int kStage = kA + kB + kSA + kSB;
-    static constexpr int kSub = OUT4 ? 0 : 32 * 32 * int(sizeof(T));  // one 32 x 32 output sub-tile
-    static constexpr int kOut = kEpiWarps * 2 * kSub;
-    static constexpr int kMax = 232448 - 1024 - 256;  // the 227 KB per CTA, less alignment slack and barriers
-    static constexpr int kFit = (kMax - kOut) / kStage;
-    static constexpr int kStages = kFit < 8 ? kFit : 8;
-    static constexpr int kBars = (2 * kStages + 5) * 8;
-    static constexpr int kSmem = 1024 + kStages * kStage + kOut + kBars + 16;
-    static_assert(kSmem <= 232448 && kStages >= 3, "shared memory over the 227 KB per-CTA limit");
-    // tensor memory columns: accumulators at 0 and kAcc1, two scale buffers (A's, then W's) at kSf
+    static constexpr int kSlots = 6;
+    static constexpr int kCW = BN / 4 > 32 ? BN / 4 : 32;  // columns per epilogue warp
+    static constexpr int kGroups = BN / kCW;                // epilogue warps per 32 rows
+    // output staging: sub-tiles of 32 rows x kSW columns, one buffer per warp
+    static constexpr int kSW = sizeof(T) == 4 ? 32 : kCW;
+    static constexpr int kSub = 32 * kSW * int(sizeof(T));
+    static constexpr int kOut = OUT4 ? 0 : kEpiWarps * kSub;
+    static constexpr int kFixed = 1024 + kOut + kSlots * (kSA + kSB) + 640;  // alignment slack, ..., barriers
+    // tensor memory columns: accumulators at 0 and kAcc1, then per stage two halves of K = 128, each with A's
+    // scales and W's
     static constexpr bool kOverlap = BN == 256;
-    static constexpr int kAcc1 = kOverlap ? 192 : BN, kSf = kAcc1 + BN, kSfBuf = 2 * 4 + 2 * 4 * kNTiles;
-    static constexpr int kCols = kSf + 2 * kSfBuf <= 256 ? 256 : 512;
-    static_assert(kSf + 2 * kSfBuf <= kCols, "tensor memory over 512 columns");
+    static constexpr int kAcc1 = kOverlap ? 128 : BN, kSf = kAcc1 + BN, kSfHalf = 4 + 4 * kNTiles, kSfBuf = 2 * kSfHalf;
+    static constexpr int kFit = (232448 - kFixed) / (kA + kB), kFitT = (512 - kSf) / kSfBuf;
+    static constexpr int kStages = kFit < kFitT ? (kFit < 8 ? kFit : 8) : (kFitT < 8 ? kFitT : 8);
+    static constexpr int kSmem = kFixed + kStages * (kA + kB);
+    static_assert(kStages >= 3, "shared memory over the 227 KB per-CTA limit");
+    static constexpr int kCols = kSf + kStages * kSfBuf <= 256 ? 256 : 512;
+    static_assert(kSf + kStages * kSfBuf <= kCols, "tensor memory over 512 columns");
+    static constexpr int kBarriers = 2 * kStages + 2 * kSlots + 2 + 2 + 1 + kEpiWarps;
+    static_assert(kBarriers * 8 + 16 <= 640, "barrier area");
 };
 
 template <class T, int BN, bool PAIR, int EPI, bool OUT4>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
-                    const __grid_constant__ CUtensorMap tmY, Params p) {
+                    const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR, Params p) {
     using L = Layout<T, BN, PAIR, OUT4>;
-    constexpr int STAGES = L::kStages;
+    constexpr int STAGES = L::kStages, SLOTS = L::kSlots;
     constexpr int UM = PAIR ? 2 * BM : BM;  // rows of one output tile (one CTA, or the pair)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sA = smem;
     uint8_t* sB = sA + STAGES * L::kA;
     uint8_t* sOut = sB + STAGES * L::kB;
-    uint8_t* sSA = sOut + L::kOut;
-    uint8_t* sSB = sSA + STAGES * L::kSA;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sSB + STAGES * L::kSB);
+    uint8_t* sSc = sOut + L::kOut;
+    // full: a stage's codes are in shared memory and its scales in tensor memory (the leader's, for both CTAs)
+    uint64_t* full = reinterpret_cast<uint64_t*>(sSc + SLOTS * (L::kSA + L::kSB));
     uint64_t* empty = full + STAGES;
-    uint64_t* tfull = empty + STAGES;
+    uint64_t* sfull = empty + STAGES;   // scale slots, in shared memory
+    uint64_t* sempty = sfull + SLOTS;
+    uint64_t* tfull = sempty + SLOTS;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* rfull = drain + 1;  // per epilogue warp: its residual sub-tile
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + kEpiWarps);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_rank() : 0u;  // 0: the pair leader (issues the MMAs)
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int b = 0; b < 2; ++b) mbar_init(&tfull[b], 1), mbar_init(&tempty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+        constexpr uint32_t ctas = PAIR ? 2 : 1;
+        for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1 + 4 * ctas), mbar_init(&empty[s], 1);
+        for (int s = 0; s < SLOTS; ++s) mbar_init(&sfull[s], 1), mbar_init(&sempty[s], 4);
+        for (int b = 0; b < 2; ++b) mbar_init(&tfull[b], 1), mbar_init(&tempty[b], 4 * L::kGroups * ctas);
         mbar_init(drain, 1);
+        for (int w = 0; w < kEpiWarps; ++w) mbar_init(&rfull[w], 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 3) {
         if (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                          "r"(L::kCols));
@@ -215,237 +256,302 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int unit0 = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
     const int units = PAIR ? int(gridDim.x >> 1) : int(gridDim.x);
 
-    if (warp == 0 && lane == 0) {
-        // ---------------- TMA producer
-        int stage = 0;
-        uint32_t phase = 0;
-        uint32_t issued = 0, last_parity = 0;  // per-stage bit masks for the drain
-        for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
-            const int mb = tile / n_n, nb = tile - mb * n_n;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        if (warp == 0 && lane == 0) {
+            // ---------------- TMA producer of the codes
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
+                const int mb = tile / n_n, nb = tile - mb * n_n;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) break;
+                    if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * (L::kA + L::kB)));
+                    load_codes<PAIR>(sA + stage * L::kA, &tmA, &full[stage], kb * BKB, mb * UM + int(rank) * BM);
+                    load_codes<PAIR>(sB + stage * L::kB, &tmW, &full[stage], kb * BKB, nb * BN + int(rank) * (BN / 2));
+                    if (++stage == STAGES) stage = 0, phase ^= 1;
+                }
+            }
+            if (*abort_flag) settle();
+        } else if (warp == 2 && lane == 0) {
+            // ---------------- TMA producer of the scales (all of the W tile's, in both CTAs of a pair)
+            int slot = 0;
+            uint32_t phase = 0;
+            for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
+                const int mb = tile / n_n, nb = tile - mb * n_n;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(&sempty[slot], phase ^ 1, abort_flag)) break;
+                    mbar_expect_tx(&sfull[slot], uint32_t(L::kSA + L::kSB));
+                    uint8_t* d = sSc + slot * (L::kSA + L::kSB);
+                    tma_load_3d(d, &tmSA, &sfull[slot], 0, kb * 2, (mb * UM) / 128 + int(rank));
+                    tma_load_3d(d + L::kSA, &tmSW, &sfull[slot], 0, kb * 2, nb * BN / 128);
+                    if (++slot == SLOTS) slot = 0, phase ^= 1;
+                }
+            }
+            if (*abort_flag) settle();
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            // ---------------- MMA issuer (the pair's leader issues for both CTAs)
+            constexpr uint32_t idesc0 = instr_desc(UM, BN, 0), idesc2 = instr_desc(UM, BN, 2);
+            int stage = 0, it = 0;
+            uint32_t phase = 0;
+            bool any = false;
+            for (int tile = unit0; tile < tiles; tile += units, ++it) {
+                if (*abort_flag) break;
+                const int ab = it & 1;
+                // the accumulator has been read: its own last tile's, or (overlapping accumulators) the
+                // previous tile's, whose readers were done with the tile before
+                if (L::kOverlap) {
+                    if (it > 0 && !mbar_wait(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag)) break;
+                } else {
+                    if (!mbar_wait(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag)) break;
+                }
+                fence_after();
+                const uint32_t d = tmem + uint32_t(ab * L::kAcc1);
+                // a 64-column tile of W uses half of a tile of 128 rows' scales
+                const uint32_t half = BN == 64 ? uint32_t((tile % n_n) & 1) * 2u : 0u;
+                bool ok = true;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    const int n_mma = min(4, p.K64 - 4 * kb);
+                    const uint64_t a0 = codes_desc(smem_u32(sA + stage * L::kA));
+                    const uint64_t b0 = codes_desc(smem_u32(sB + stage * L::kB));
+                    const uint32_t sf = tmem + uint32_t(L::kSf + stage * L::kSfBuf);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t sa = sf + uint32_t((j >> 1) * L::kSfHalf);
+                        if (j < n_mma)
+                            mma<PAIR>(d, a0 + uint64_t(2 * j), b0 + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0, sa, sa + 4 + half,
+                                      (kb | j) != 0 ? 1u : 0u);
+                    }
+                    if (PAIR) mma_commit_pair(&empty[stage]);
+                    else mma_commit(&empty[stage]);
+                    any = true;
+                    if (++stage == STAGES) stage = 0, phase ^= 1;
+                }
+                if (!ok) break;
+                if (PAIR) mma_commit_pair(&tfull[ab]);
+                else mma_commit(&tfull[ab]);
+            }
+            if (any) {  // every MMA issued by this thread completes before the tensor memory is freed
+                if (PAIR) mma_commit_pair_local(drain);
+                else mma_commit(drain);
+                mbar_drain(drain, 0);
+            }
+        }
+    } else if (warp < kEpiWarp0) {
+        // ---------------- scales: shared memory -> this warp's lane quarter of tensor memory
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        const uint32_t tq = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(L::kSf);
+        int slot = 0, stage = 0;
+        uint32_t sphase = 0, phase = 0;
+        bool ok = true;
+        for (int tile = unit0; ok && tile < tiles; tile += units) {
             for (int kb = 0; kb < kblocks; ++kb) {
-                if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) break;
-                // a pair's copies complete on the leader's barrier, which expects both CTAs' bytes
-                if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * L::kStage));
-                const uint32_t fb = PAIR ? mapa(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
-                load_2d<PAIR>(sA + stage * L::kA, &tmA, fb, kb * BKB, mb * UM + int(rank) * BM);
-                load_2d<PAIR>(sB + stage * L::kB, &tmW, fb, kb * BKB, nb * BN + int(rank) * (BN / 2));
-                load_3d<PAIR>(sSA + stage * L::kSA, &tmSA, fb, 0, kb * 2, (mb * UM) / 128 + int(rank));
-                load_3d<PAIR>(sSB + stage * L::kSB, &tmSW, fb, 0, kb * 2, nb * BN / 128);  // all of W's, in both CTAs
-                issued |= 1u << stage;
-                last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-                if (++stage == STAGES) stage = 0, phase ^= 1;
-            }
-        }
-        if (*abort_flag) {  // let every load already issued land before the CTA exits
-            if (rank == 0) {
-                for (int s = 0; s < STAGES; ++s)
-                    if (issued & (1u << s)) mbar_drain(&full[s], (last_parity >> s) & 1);
-            } else {  // the peer's loads complete on the leader's barriers: give them time to land
-                const uint64_t t0 = now_ns();
-                while (now_ns() - t0 < 2000000ull) {
+                if (!mbar_wait(&sfull[slot], sphase, abort_flag)) {
+                    ok = false;
+                    break;
                 }
-            }
-        }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---------------- MMA issuer (the pair's leader issues for both CTAs)
-        constexpr uint32_t idesc0 = instr_desc(UM, BN, 0), idesc2 = instr_desc(UM, BN, 2);
-        int stage = 0, it = 0;
-        uint32_t phase = 0;
-        int c = 0;  // stages so far
-        bool any = false;
-        for (int tile = unit0; tile < tiles; tile += units, ++it) {
-            if (*abort_flag) break;
-            const int ab = it & 1;
-            // the accumulator is free: its own last reader is done, or (overlapping accumulators) the
-            // previous tile's epilogue has read the shared columns, after it had read all of the tile before
-            if (L::kOverlap) {
-                if (it > 0 && !mbar_wait(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag)) break;
-            } else {
-                if (!mbar_wait(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag)) break;
-            }
-            fence_after();
-            const uint32_t d = tmem + uint32_t(ab * L::kAcc1);
-            // a 64-column tile of W uses half of a tile of 128 rows' scales
-            const uint32_t half = BN == 64 ? uint32_t((tile % n_n) & 1) * 2u : 0u;
-            bool ok = true;
-            for (int kb = 0; kb < kblocks; ++kb, ++c) {
-                // the scale buffer's last readers, two stages ago, are done (their commit freed that stage)
-                if (c >= 2) {
-                    const int u = c - 2;
-                    if (!mbar_wait(&empty[u % STAGES], uint32_t(u / STAGES) & 1u, abort_flag)) ok = false;
+                // both halves (a cut last stage's second half may hold no columns of K: it is then not used)
+                const uint8_t* src = sSc + slot * (L::kSA + L::kSB) + lane * 16;
+                uint4 v[2][1 + L::kNTiles];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    v[j][0] = *reinterpret_cast<const uint4*>(src + j * 512);
+#pragma unroll
+                    for (int t = 0; t < L::kNTiles; ++t) v[j][1 + t] = *reinterpret_cast<const uint4*>(src + L::kSA + (2 * t + j) * 512);
                 }
-                if (!ok || !mbar_wait(&full[stage], phase, abort_flag)) {
+                if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {  // the MMAs that read this buffer are done
                     ok = false;
                     break;
                 }
                 fence_after();
-                const int n_mma = min(4, p.K64 - 4 * kb);
-                const uint32_t sf = tmem + uint32_t(L::kSf + (c & 1) * L::kSfBuf), sfw = sf + 8;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (2 * j >= n_mma) break;
-                    copy_scales<PAIR>(sf + 4 * j, scales_desc(smem_u32(sSA + stage * L::kSA + j * 512)));
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int t = 0; t < L::kNTiles; ++t)
-                        copy_scales<PAIR>(sfw + 4 * (j * L::kNTiles + t),
-                                          scales_desc(smem_u32(sSB + stage * L::kSB + (2 * t + j) * 512)));
+                    for (int t = 0; t <= L::kNTiles; ++t)
+                        st_scales(tq + uint32_t(stage * L::kSfBuf + j * L::kSfHalf + 4 * t), v[j][t]);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_peer(mapa(smem_u32(&full[stage]), 0));
+                    else mbar_arrive(&full[stage]);
+                    mbar_arrive(&sempty[slot]);
                 }
-                const uint64_t a0 = codes_desc(smem_u32(sA + stage * L::kA));
-                const uint64_t b0 = codes_desc(smem_u32(sB + stage * L::kB));
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < n_mma)
-                        mma<PAIR>(d, a0 + uint64_t(2 * j), b0 + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0, sf + 4 * (j >> 1),
-                                  sfw + 4 * L::kNTiles * (j >> 1) + half, (kb | j) != 0 ? 1u : 0u);
-                if (PAIR) mma_commit_pair(&empty[stage]);
-                else mma_commit(&empty[stage]);
-                any = true;
+                if (++slot == SLOTS) slot = 0, sphase ^= 1;
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }
-            if (!ok) break;
-            if (PAIR) mma_commit_pair(&tfull[ab]);
-            else mma_commit(&tfull[ab]);
         }
-        if (any) {  // every MMA and copy issued by this thread completes before the tensor memory is freed
-            if (PAIR) mma_commit_pair_local(drain);
-            else mma_commit(drain);
-            mbar_drain(drain, 0);
-        }
-    } else if (warp >= 2) {
+    } else {
         // ---------------- epilogue
-        const int ew = warp - 2;
-        const int lg = warp & 3;   // the lane quarter this warp may access: rows 32 lg .. + 31
-        const int half = ew >> 2;  // which half of the chunks
-        constexpr int kChunks = BN / 64;  // 32-column chunks per warp
-        uint8_t* obuf = sOut + ew * 2 * L::kSub;
-        uint32_t n_out = 0;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+        const int ew = warp - kEpiWarp0;
+        const int lg = warp & 3;  // the lane quarter this warp may access: rows 32 lg .. + 31
+        const int grp = ew >> 2;  // its columns: grp kCW .. + kCW - 1
+        uint8_t* ob = sOut + ew * L::kSub;
+        uint64_t* rbar = &rfull[ew];
+        uint32_t rphase = 0;
         const T* bias = static_cast<const T*>(p.bias);
-        const T* R = static_cast<const T*>(p.R);
         const uint32_t te0 = PAIR ? mapa(smem_u32(&tempty[0]), 0) : 0u, te1 = PAIR ? mapa(smem_u32(&tempty[1]), 0) : 0u;
-        auto release = [&](int ab) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR) mbar_arrive_cluster(ab ? te1 : te0);
-                else mbar_arrive(&tempty[ab]);
-            }
+        // 16-byte chunk j of row r of a staged sub-tile, swizzled as the tensor map has it
+        auto chunk_at = [&](int r, int j) -> uint8_t* {
+            return ob + (L::kSW * sizeof(T) == 128 ? r * 128 + ((j ^ (r & 7)) << 4) : sw64(r, j));
         };
-        // the chunk of the tile that this warp takes as its c-th: with overlapping accumulators the shared
-        // columns first (chunks 6 and 7 of the first, 0 and 1 of the second)
-        auto chunk_of = [&](int ab, int c) -> int {
-            if (!L::kOverlap) return half * kChunks + c;
-            if (c == 0) return (ab ? 0 : 6) + half;
-            return (ab ? 2 : 0) + half * 3 + c - 1;
+        // one lane: the residual sub-tile into the staging buffer, once the store before has read that
+        auto load_residual = [&](int col0, int row0) {
+            bulk_wait_read0();
+            mbar_expect_tx(rbar, uint32_t(L::kSub));
+            tma_load_2d(ob, &tmR, rbar, col0, row0);
         };
         int it = 0;
-        for (int tile = unit0; tile < tiles; tile += units, ++it) {
+        for (int tile = unit0; grp < L::kGroups && tile < tiles; tile += units, ++it) {
             const int ab = it & 1;
             const int mb = tile / n_n, nb = tile - mb * n_n;
             const int row0 = mb * UM + int(rank) * BM + lg * 32, row = row0 + lane;
-            if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag)) break;
+            const int colw = nb * BN + grp * L::kCW;
+            if (EPI == k::kEpiResidual) {
+                __syncwarp();  // every lane is done with the buffer
+                if (lane == 0) load_residual(colw, row0);
+            }
+            if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag)) {
+                if (EPI == k::kEpiResidual && lane == 0) mbar_drain(rbar, rphase);
+                break;
+            }
             fence_after();
-            const uint32_t taddr = tmem + (uint32_t(lg * 32) << 16) + uint32_t(ab * L::kAcc1);
-            uint32_t ra[32], rb[32];
-            tmem_ld32_async(taddr + uint32_t(32 * chunk_of(ab, 0)), ra);
-            tmem_wait32(ra);
-            if (L::kOverlap || kChunks == 1) release(ab);
+            const uint32_t taddr = tmem + (uint32_t(lg * 32) << 16) + uint32_t(ab * L::kAcc1 + grp * L::kCW);
+            uint32_t acc[L::kCW / 32][32];
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                uint32_t(&cur)[32] = (c & 1) ? rb : ra;
-                uint32_t(&nxt)[32] = (c & 1) ? ra : rb;
-                const int col0 = nb * BN + 32 * chunk_of(ab, c);
-                if (c + 1 < kChunks) tmem_ld32_async(taddr + uint32_t(32 * chunk_of(ab, c + 1)), nxt);
-                float v[32];
+            for (int c = 0; c < L::kCW / 32; ++c) tmem_ld32_async(taddr + uint32_t(32 * c), acc[c]);
+#pragma unroll
+            for (int c = 0; c < L::kCW / 32; ++c) tmem_wait32(acc[c]);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_peer(ab ? te1 : te0);
+                else mbar_arrive(&tempty[ab]);
+            }
+            uint32_t scales = 0;  // OUT4: the scale bytes of the warp's columns
+#pragma unroll
+            for (int c = 0; c < L::kCW / 32; ++c) {
+                const int col0 = colw + 32 * c;
                 const bool whole = col0 + 32 <= p.N;
-                if (bias && whole) {
+                float v[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(cur[i]) + to_f<T>(__ldg(bias + col0 + i));
-                } else {
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[c][i]);
+                if (bias) {
+                    if (whole && p.bias16) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        v[i] = __uint_as_float(cur[i]) + (bias && col0 + i < p.N ? to_f<T>(bias[col0 + i]) : 0.0f);
+                        for (int i = 0; i < 32; i += 8) {
+                            float b[8];
+                            Vec<T, 8>::ldg(bias + col0 + i, b);
+#pragma unroll
+                            for (int j = 0; j < 8; j += 2) {
+                                const float2 s = __fadd2_rn(make_float2(v[i + j], v[i + j + 1]), make_float2(b[j], b[j + 1]));
+                                v[i + j] = s.x, v[i + j + 1] = s.y;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (col0 + i < p.N) v[i] += to_f<T>(bias[col0 + i]);
+                    }
                 }
                 if (EPI == k::kEpiGelu) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 g = p.gelu_tanh ? make_float2(gelu(v[i], true), gelu(v[i + 1], true))
-                                                     : gelu_as2(make_float2(v[i], v[i + 1]));
+                                                     : gelu2(make_float2(v[i], v[i + 1]));
                         v[i] = g.x, v[i + 1] = g.y;
                     }
                 }
-                if (EPI == k::kEpiResidual && row < p.M) {
-                    const T* r = R + int64_t(row) * p.ldr + col0;
-                    if (whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float b[8];
-                            Vec<T, 8>::load(r + i, b);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) v[i + j] += b[j];
-                        }
-                    } else {
+                if constexpr (OUT4) {
+                    if (!whole) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (col0 + i < p.N) v[i] += to_f<T>(r[i]);
+                            if (col0 + i >= p.N) v[i] = 0.0f;
                     }
-                }
-                if (c + 1 < kChunks) {
-                    tmem_wait32(nxt);
-                    if (!L::kOverlap && c + 2 == kChunks) release(ab);  // every column is in registers
-                }
-                if (OUT4) {
-                    if (row < p.M && col0 < p.N) {
-                        uint32_t top = 0;
+                    uint32_t top = 0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (!whole && col0 + i >= p.N) v[i] = 0.0f;
-                            top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-                        }
-                        const uint32_t s = scale_byte(top);
-                        const float inv = inv_scale(s);
+                    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                    const uint32_t s = scale_byte(top);
+                    const float inv = inv_scale(s);
+                    scales |= s << (8 * c);
+                    if (row < p.M && col0 < p.N)
                         *reinterpret_cast<uint4*>(p.Yc + int64_t(row) * p.ldyc + col0 / 2) =
                             make_uint4(encode8(v, inv), encode8(v + 8, inv), encode8(v + 16, inv), encode8(v + 24, inv));
-                        p.Ys[scale_at(row, col0 / 32, p.ktiles_out)] = uint8_t(s);
-                    } else if (row < p.M && col0 / 32 < int(4 * p.ktiles_out)) {
-                        p.Ys[scale_at(row, col0 / 32, p.ktiles_out)] = 0;  // the last scale tile's blocks past N
-                    }
-                    // (a 64-column tile that is the first half of the last scale tile: its second half)
-                    if (BN == 64 && row < p.M && nb == n_n - 1 && !(nb & 1))
-                        p.Ys[scale_at(row, col0 / 32 + 2, p.ktiles_out)] = 0;
-                } else if (!whole && (p.N * int(sizeof(T))) % 16 != 0) {
-                    // a TMA store writes whole 16-byte pieces: the columns past N belong to the caller
-                    if (row < p.M) {
-                        T* y = static_cast<T*>(p.Y) + int64_t(row) * p.ldy + col0;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (col0 + i < p.N) y[i] = from_f<T>(v[i]);
-                    }
                 } else {
-                    const uint32_t obi = n_out & 1;
-                    if (n_out >= 2 && lane == 0) bulk_wait_read1();  // the store that used this buffer read it
-                    __syncwarp();
-                    uint8_t* ob = obuf + obi * L::kSub;
-                    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[i] = pack_h2(make_float2(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]));
-                            *reinterpret_cast<uint4*>(ob + sw64(lane, j)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    constexpr int kChunks = 32 * int(sizeof(T)) / 16;  // 16-byte chunks of the 32 columns
+                    constexpr int kVals = 16 / int(sizeof(T));
+                    const int j0 = L::kSW == 64 ? 4 * c : 0;
+                    if (EPI == k::kEpiResidual) {
+                        if (L::kSW == 32 && c > 0) {  // a second sub-tile through the same buffer
+                            __syncwarp();
+                            if (lane == 0) load_residual(col0, row0);
                         }
-                    } else {
+                        if (L::kSW == 32 || c == 0) {
+                            if (!mbar_wait(rbar, rphase, abort_flag)) {
+                                if (lane == 0) mbar_drain(rbar, rphase);
+                                __syncwarp();
+                            }
+                            rphase ^= 1;
+                        }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<float4*>(ob + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        for (int j = 0; j < kChunks; ++j) {
+                            float r[kVals];
+                            Vec<T, kVals>::load(reinterpret_cast<const T*>(chunk_at(lane, j0 + j)), r);
+#pragma unroll
+                            for (int i = 0; i < kVals; ++i) v[kVals * j + i] += r[i];
+                        }
+                    } else if (L::kSW == 32 || c == 0) {
+                        if (lane == 0) bulk_wait_read0();  // the store before has read the buffer
+                        __syncwarp();
                     }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (col0 < p.N && row0 < p.M) tma_store_2d(&tmY, ob, col0, row0);  // (rows past M are clipped)
-                        bulk_commit();
+                    // a TMA store writes whole 16-byte pieces: a row's columns past N belong to the caller
+                    const bool ragged = colw + L::kCW > p.N && (p.N * int(sizeof(T))) % 16 != 0;
+                    if (ragged) {
+                        if (row < p.M) {
+                            T* y = static_cast<T*>(p.Y) + int64_t(row) * p.ldy + col0;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (col0 + i < p.N) y[i] = from_f<T>(v[i]);
+                        }
+                        continue;
                     }
-                    ++n_out;
+#pragma unroll
+                    for (int j = 0; j < kChunks; ++j) {
+                        uint4 o;
+                        if constexpr (sizeof(T) == 2)
+                            o = make_uint4(pack_h2(make_float2(v[8 * j], v[8 * j + 1])), pack_h2(make_float2(v[8 * j + 2], v[8 * j + 3])),
+                                           pack_h2(make_float2(v[8 * j + 4], v[8 * j + 5])), pack_h2(make_float2(v[8 * j + 6], v[8 * j + 7])));
+                        else
+                            o = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                                           __float_as_uint(v[4 * j + 3]));
+                        *reinterpret_cast<uint4*>(chunk_at(lane, j0 + j)) = o;
+                    }
+                    if (L::kSW == 32 || c + 1 == L::kCW / 32) {
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const int cs = L::kSW == 32 ? col0 : colw;
+                            if (cs < p.N && row0 < p.M) tma_store_2d(&tmY, ob, cs, row0);  // (past M and N: clipped)
+                            bulk_commit();
+                        }
+                    }
+                }
+            }
+            if constexpr (OUT4) {
+                // the blocks' scale bytes; 0 for the last scale tile's blocks past N
+                const int b0 = colw / 32;
+                if (row < p.M && b0 < int(4 * p.ktiles_out)) {
+                    uint8_t* d = p.Ys + scale_at(row, b0, p.ktiles_out);
+                    if (L::kCW == 64) *reinterpret_cast<uint16_t*>(d) = uint16_t(scales);
+                    else *d = uint8_t(scales);
+                    // (a 64-column tile that is the first half of the last scale tile: its second half)
+                    if (BN == 64 && nb == n_n - 1 && !(nb & 1)) d[2] = 0;
                 }
             }
         }
@@ -455,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before();
     __syncthreads();
     if (PAIR) cluster_sync();  // no CTA leaves while its peer may still read its shared memory or signal it
-    if (warp == 1) {
+    if (warp == 3) {
         fence_after();
         if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols));
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols));
@@ -476,32 +582,42 @@ CUtensorMap scales_map(const uint8_t* base, int64_t rows, int64_t ktiles, int bo
     return tc::tensor_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Rows of the output or residual, box [32, width], 128 or 64 bytes wide and swizzled so.
+template <class T> CUtensorMap rows_map(const T* base, int64_t rows, int64_t cols, int64_t ld, int width) {
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * sizeof(T)};
+    const cuuint32_t box[2] = {cuuint32_t(width), 32};
+    return tc::tensor_map(base, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, dims,
+                          strides, box, width * sizeof(T) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const GemmArgs<T>& a, cudaStream_t s) {
     using L = Layout<T, BN, PAIR, OUT4>;
     static std::atomic<uint64_t> configured{0};  // per instantiation and device
     once_per_device(configured, [] {
-        VB_CUDA(cudaFuncSetAttribute(gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     L::kSmem));
+        auto* kernel = &gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4>;
+        VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+        // the epilogue's registers come out of what the CTA is launched with
+        cudaFuncAttributes f{};
+        VB_CUDA(cudaFuncGetAttributes(&f, kernel));
+        if (f.numRegs < kLaunchRegs) fail(kInternal, "gemm_mx4: built with fewer registers per thread than it splits");
     });
     const int64_t kt = k_tiles(a.K);
     const CUtensorMap ta = codes_map(a.A, a.M, row_bytes(a.K), a.lda, BM);
     const CUtensorMap tw = codes_map(a.W, a.N, row_bytes(a.K), a.ldw, PAIR ? BN / 2 : BN);
     const CUtensorMap tsa = scales_map(a.sA, a.M, kt, 1), tsw = scales_map(a.sW, a.N, kt, L::kNTiles);
-    CUtensorMap ty = ta;
+    CUtensorMap ty = ta, tr = ta;
     if (!OUT4) {
-        const cuuint64_t dims[2] = {cuuint64_t(a.N), cuuint64_t(a.M)}, strides[1] = {cuuint64_t(a.ldy) * sizeof(T)};
-        const cuuint32_t box[2] = {32, 32};
-        ty = tc::tensor_map(a.Y, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, dims,
-                            strides, box, sizeof(T) == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+        ty = rows_map(a.Y, a.M, a.N, a.ldy, L::kSW);
+        if (EPI == k::kEpiResidual) tr = rows_map(a.R, a.M, a.N, a.ldr, L::kSW);
     }
     const Params p{a.bias, a.R, a.ldr, a.Y, a.ldy, a.Yc, a.ldyc, a.Ys, k_tiles(a.N), int(a.M), int(a.N), int((a.K + 63) / 64),
-                   a.gelu_tanh ? 1 : 0};
+                   a.gelu_tanh ? 1 : 0, (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0 ? 1 : 0};
     constexpr int UM = PAIR ? 2 * BM : BM;
     const int64_t tiles = ((a.M + UM - 1) / UM) * ((a.N + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) fail(kUnsupported, "gemm_mx4: too many output tiles");
     if (!PAIR) {
         const int grid = int(std::min<int64_t>(tiles, device_sm_count()));
-        gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4><<<grid, kThreads, L::kSmem, s>>>(ta, tw, tsa, tsw, ty, p);
+        gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4><<<grid, kThreads, L::kSmem, s>>>(ta, tw, tsa, tsw, ty, tr, p);
         VB_LAUNCH();
         return;
     }
@@ -515,7 +631,7 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    VB_CUDA(cudaLaunchKernelEx(&cfg, gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4>, ta, tw, tsa, tsw, ty, p));
+    VB_CUDA(cudaLaunchKernelEx(&cfg, gemm_mx4_kernel<T, BN, PAIR, EPI, OUT4>, ta, tw, tsa, tsw, ty, tr, p));
     ++launch_counter();
 }
 
