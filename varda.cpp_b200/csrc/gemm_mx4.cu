@@ -461,11 +461,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (EPI == k::kEpiGelu) {
+                    if (p.gelu_tanh) {
+#pragma unroll 1
+                        for (int i = 0; i < 32; ++i) {
+                            // (a rotation, so that the registers are not indexed and the code stays small)
+                            const float g = gelu(v[0], true);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 g = p.gelu_tanh ? make_float2(gelu(v[i], true), gelu(v[i + 1], true))
-                                                     : gelu2(make_float2(v[i], v[i + 1]));
-                        v[i] = g.x, v[i + 1] = g.y;
+                            for (int j = 0; j < 31; ++j) v[j] = v[j + 1];
+                            v[31] = g;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 g = gelu2(make_float2(v[i], v[i + 1]));
+                            v[i] = g.x, v[i + 1] = g.y;
+                        }
                     }
                 }
                 if constexpr (OUT4) {
