@@ -105,7 +105,8 @@ class _LazyLib:
         return _LazyLib._handle
 
     def __getattr__(self, name):
-        return getattr(self.get(), name)
+        f = self.__dict__[name] = getattr(self.get(), name)  # found at once from the second call on
+        return f
 
 
 lib = _LazyLib()
@@ -135,13 +136,13 @@ STEP = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.POINTER(ctypes.c_float), ctyp
 
 
 def _ptr(a):
-    if a is None:
-        return None
-    if isinstance(a, int):
-        return ctypes.c_void_p(a)
-    if hasattr(a, "data_ptr"):  # torch tensor (device memory plumbing)
-        return ctypes.c_void_p(a.data_ptr())
-    return a.ctypes.data_as(ctypes.c_void_p)
+    """The address of a device tensor or host array, for a c_void_p argument (None and integers are passed on)."""
+    if a is None or type(a) is int:
+        return a
+    try:
+        return a.data_ptr()  # torch tensor (device memory plumbing)
+    except AttributeError:
+        return a.ctypes.data_as(ctypes.c_void_p)
 
 
 def _check_out(a, n, what):
