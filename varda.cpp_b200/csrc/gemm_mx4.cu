@@ -63,7 +63,6 @@ struct Params {
     int64_t ktiles_out;
     int M, N, K64;  // K64: MMAs along K, ceil(K / 64)
     int gelu_tanh;
-    int bias16;  // bias is 16-byte aligned
 };
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
@@ -181,7 +180,8 @@ template <class T, int BN, bool PAIR, bool OUT4> struct Layout {
     static constexpr int kSW = sizeof(T) == 4 ? 32 : kCW;
     static constexpr int kSub = 32 * kSW * int(sizeof(T));
     static constexpr int kOut = OUT4 ? 0 : kEpiWarps * kSub;
-    static constexpr int kFixed = 1024 + kOut + kSlots * (kSA + kSB) + 640;  // alignment slack, ..., barriers
+    static constexpr int kBias = kEpiWarps * kCW * 4;  // each epilogue warp's columns of the bias, fp32
+    static constexpr int kFixed = 1024 + kOut + kSlots * (kSA + kSB) + kBias + 640;  // alignment slack, ..., barriers
     // tensor memory columns: accumulators at 0 and kAcc1, then per stage two halves of K = 128, each with A's
     // scales and W's
     static constexpr bool kOverlap = BN == 256;
@@ -210,8 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* sB = sA + STAGES * L::kA;
     uint8_t* sOut = sB + STAGES * L::kB;
     uint8_t* sSc = sOut + L::kOut;
+    float* sBias = reinterpret_cast<float*>(sSc + SLOTS * (L::kSA + L::kSB));
     // full: a stage's codes are in shared memory and its scales in tensor memory (the leader's, for both CTAs)
-    uint64_t* full = reinterpret_cast<uint64_t*>(sSc + SLOTS * (L::kSA + L::kSB));
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sBias) + L::kBias);
     uint64_t* empty = full + STAGES;
     uint64_t* sfull = empty + STAGES;   // scale slots, in shared memory
     uint64_t* sempty = sfull + SLOTS;
@@ -393,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int lg = warp & 3;  // the lane quarter this warp may access: rows 32 lg .. + 31
         const int grp = ew >> 2;  // its columns: grp kCW .. + kCW - 1
         uint8_t* ob = sOut + ew * L::kSub;
+        float* wb = sBias + ew * L::kCW;
         uint64_t* rbar = &rfull[ew];
         uint32_t rphase = 0;
         const T* bias = static_cast<const T*>(p.bias);
@@ -413,10 +415,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int mb = tile / n_n, nb = tile - mb * n_n;
             const int row0 = mb * UM + int(rank) * BM + lg * 32, row = row0 + lane;
             const int colw = nb * BN + grp * L::kCW;
-            if (EPI == k::kEpiResidual) {
-                __syncwarp();  // every lane is done with the buffer
-                if (lane == 0) load_residual(colw, row0);
-            }
+            __syncwarp();  // every lane is done with the tile before's buffers
+            if (EPI == k::kEpiResidual && lane == 0) load_residual(colw, row0);
+#pragma unroll
+            for (int i = lane; i < L::kCW; i += 32) wb[i] = bias && colw + i < p.N ? to_f<T>(__ldg(bias + colw + i)) : 0.0f;
+            __syncwarp();
             if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag)) {
                 if (EPI == k::kEpiResidual && lane == 0) mbar_drain(rbar, rphase);
                 break;
@@ -441,24 +444,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool whole = col0 + 32 <= p.N;
                 float v[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[c][i]);
-                if (bias) {
-                    if (whole && p.bias16) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float b[8];
-                            Vec<T, 8>::ldg(bias + col0 + i, b);
-#pragma unroll
-                            for (int j = 0; j < 8; j += 2) {
-                                const float2 s = __fadd2_rn(make_float2(v[i + j], v[i + j + 1]), make_float2(b[j], b[j + 1]));
-                                v[i + j] = s.x, v[i + j + 1] = s.y;
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (col0 + i < p.N) v[i] += to_f<T>(bias[col0 + i]);
-                    }
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(wb + 32 * c + i);
+                    const float2 s0 = __fadd2_rn(make_float2(__uint_as_float(acc[c][i]), __uint_as_float(acc[c][i + 1])), make_float2(b.x, b.y));
+                    const float2 s1 = __fadd2_rn(make_float2(__uint_as_float(acc[c][i + 2]), __uint_as_float(acc[c][i + 3])), make_float2(b.z, b.w));
+                    v[i] = s0.x, v[i + 1] = s0.y, v[i + 2] = s1.x, v[i + 3] = s1.y;
                 }
                 if (EPI == k::kEpiGelu) {
                     if (p.gelu_tanh) {
@@ -484,10 +474,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 32; ++i)
                             if (col0 + i >= p.N) v[i] = 0.0f;
                     }
-                    uint32_t top = 0;
+                    float top = 0.0f;  // NaN if one is
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-                    const uint32_t s = scale_byte(top);
+                    for (int i = 0; i < 32; i += 2)
+                        asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+                    const uint32_t s = scale_byte(__float_as_uint(top) & 0x7fffffffu);
                     const float inv = inv_scale(s);
                     scales |= s << (8 * c);
                     if (row < p.M && col0 < p.N)
@@ -621,7 +612,7 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
         if (EPI == k::kEpiResidual) tr = rows_map(a.R, a.M, a.N, a.ldr, L::kSW);
     }
     const Params p{a.bias, a.R, a.ldr, a.Y, a.ldy, a.Yc, a.ldyc, a.Ys, k_tiles(a.N), int(a.M), int(a.N), int((a.K + 63) / 64),
-                   a.gelu_tanh ? 1 : 0, (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0 ? 1 : 0};
+                   a.gelu_tanh ? 1 : 0};
     constexpr int UM = PAIR ? 2 * BM : BM;
     const int64_t tiles = ((a.M + UM - 1) / UM) * ((a.N + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) fail(kUnsupported, "gemm_mx4: too many output tiles");

@@ -55,6 +55,9 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
 // Eight codes (column i in bits 4i .. 4i + 3) of v[i] * inv; 0 for a NaN block.
 __device__ __forceinline__ uint32_t encode8(const float* v, float inv) {
     uint32_t d;
+    float2 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(inv, inv));
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -62,8 +65,7 @@ __device__ __forceinline__ uint32_t encode8(const float* v, float inv) {
         "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
         "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(d)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
-          "f"(v[6] * inv), "f"(v[7] * inv));
+        : "f"(s[0].x), "f"(s[0].y), "f"(s[1].x), "f"(s[1].y), "f"(s[2].x), "f"(s[2].y), "f"(s[3].x), "f"(s[3].y));
     return inv == 0.0f ? 0u : d;
 }
 // The eight e2m1 values of a word of codes.
