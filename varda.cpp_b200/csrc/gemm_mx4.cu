@@ -639,8 +639,9 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
 template <class T, int EPI, bool OUT4> void dispatch_tile(const GemmArgs<T>& a, cudaStream_t s) {
     auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
     const int64_t sms = device_sm_count();
-    // the largest tile that still gives every SM (pair) one
-    if (tiles(256, 256) >= sms / 2) launch<T, 256, true, EPI, OUT4>(a, s);
+    // the largest tile that still gives every SM (pair) one, and no wider than N ([40321 x 1024] x [1024 x 80]: 11 us,
+    // with 256-column tiles 17)
+    if (a.N > 128 && tiles(256, 256) >= sms / 2) launch<T, 256, true, EPI, OUT4>(a, s);
     else if (tiles(128, 128) >= sms) launch<T, 128, false, EPI, OUT4>(a, s);
     else launch<T, 64, false, EPI, OUT4>(a, s);
 }
