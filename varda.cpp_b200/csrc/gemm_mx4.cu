@@ -44,8 +44,8 @@ using namespace vb::ptx;
 
 constexpr int BM = 128, BKB = 128;  // rows of a CTA's tile; bytes of codes per row and stage (256 columns)
 constexpr int kEpiWarps = 16, kEpiWarp0 = 8, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-// registers: the first two warpgroups give back to the epilogue's four (2 x 40 + 4 x 96 <= 6 x the 80 of the launch)
-constexpr int kLaunchRegs = 80, kFewRegs = 40, kEpiRegs = 96;
+// registers: the first two warpgroups give back to the epilogue's four (2 x 48 + 4 x 96 <= 6 x the 80 of the launch)
+constexpr int kLaunchRegs = 80, kFewRegs = 48, kEpiRegs = 96;
 static_assert(2 * kFewRegs + 4 * kEpiRegs <= 6 * kLaunchRegs, "register split over what the CTA is launched with");
 constexpr unsigned long long kTimeoutNs = 4000000000ull;  // 4 s
 
@@ -130,6 +130,11 @@ __device__ __forceinline__ void st_scales(uint32_t taddr, uint4 v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
                  "r"(v.w)
                  : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
@@ -290,8 +295,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (*abort_flag) settle();
-        } else if (warp == 1 && lane == 0 && rank == 0) {
-            // ---------------- MMA issuer (the pair's leader issues for both CTAs)
+        } else if (warp == 1 && rank == 0) {
+            // ---------------- MMA issuer (the pair's leader issues for both CTAs). The whole warp runs the loop and one
+            // lane issues, so that descriptors and addresses are uniform values
+            const bool leader = elect_one();
             constexpr uint32_t idesc0 = instr_desc(UM, BN, 0), idesc2 = instr_desc(UM, BN, 2);
             int stage = 0, it = 0;
             uint32_t phase = 0;
@@ -321,23 +328,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t a0 = codes_desc(smem_u32(sA + stage * L::kA));
                     const uint64_t b0 = codes_desc(smem_u32(sB + stage * L::kB));
                     const uint32_t sf = tmem + uint32_t(L::kSf + stage * L::kSfBuf);
+                    if (leader) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t sa = sf + uint32_t((j >> 1) * L::kSfHalf);
-                        if (j < n_mma)
-                            mma<PAIR>(d, a0 + uint64_t(2 * j), b0 + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0, sa, sa + 4 + half,
-                                      (kb | j) != 0 ? 1u : 0u);
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t sa = sf + uint32_t((j >> 1) * L::kSfHalf);
+                            if (j < n_mma)
+                                mma<PAIR>(d, a0 + uint64_t(2 * j), b0 + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0, sa, sa + 4 + half,
+                                          (kb | j) != 0 ? 1u : 0u);
+                        }
+                        if (PAIR) mma_commit_pair(&empty[stage]);
+                        else mma_commit(&empty[stage]);
                     }
-                    if (PAIR) mma_commit_pair(&empty[stage]);
-                    else mma_commit(&empty[stage]);
+                    __syncwarp();
                     any = true;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
                 if (!ok) break;
-                if (PAIR) mma_commit_pair(&tfull[ab]);
-                else mma_commit(&tfull[ab]);
+                if (leader) {
+                    if (PAIR) mma_commit_pair(&tfull[ab]);
+                    else mma_commit(&tfull[ab]);
+                }
+                __syncwarp();
             }
-            if (any) {  // every MMA issued by this thread completes before the tensor memory is freed
+            if (any && leader) {  // every MMA issued by this thread completes before the tensor memory is freed
                 if (PAIR) mma_commit_pair_local(drain);
                 else mma_commit(drain);
                 mbar_drain(drain, 0);
