@@ -264,33 +264,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-        if (warp == 0 && lane == 0) {
+        if (warp == 0) {
             // ---------------- TMA producer of the codes
+            const bool leader = elect_one();
             int stage = 0;
             uint32_t phase = 0;
             for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) break;
-                    if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * (L::kA + L::kB)));
-                    load_codes<PAIR>(sA + stage * L::kA, &tmA, &full[stage], kb * BKB, mb * UM + int(rank) * BM);
-                    load_codes<PAIR>(sB + stage * L::kB, &tmW, &full[stage], kb * BKB, nb * BN + int(rank) * (BN / 2));
+                    if (leader) {
+                        if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * (L::kA + L::kB)));
+                        load_codes<PAIR>(sA + stage * L::kA, &tmA, &full[stage], kb * BKB, mb * UM + int(rank) * BM);
+                        load_codes<PAIR>(sB + stage * L::kB, &tmW, &full[stage], kb * BKB, nb * BN + int(rank) * (BN / 2));
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
             }
             if (*abort_flag) settle();
-        } else if (warp == 2 && lane == 0) {
+        } else if (warp == 2) {
             // ---------------- TMA producer of the scales (all of the W tile's, in both CTAs of a pair)
+            const bool leader = elect_one();
             int slot = 0;
             uint32_t phase = 0;
             for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&sempty[slot], phase ^ 1, abort_flag)) break;
-                    mbar_expect_tx(&sfull[slot], uint32_t(L::kSA + L::kSB));
-                    uint8_t* d = sSc + slot * (L::kSA + L::kSB);
-                    tma_load_3d(d, &tmSA, &sfull[slot], 0, kb * 2, (mb * UM) / 128 + int(rank));
-                    tma_load_3d(d + L::kSA, &tmSW, &sfull[slot], 0, kb * 2, nb * BN / 128);
+                    if (leader) {
+                        mbar_expect_tx(&sfull[slot], uint32_t(L::kSA + L::kSB));
+                        uint8_t* d = sSc + slot * (L::kSA + L::kSB);
+                        tma_load_3d(d, &tmSA, &sfull[slot], 0, kb * 2, (mb * UM) / 128 + int(rank));
+                        tma_load_3d(d + L::kSA, &tmSW, &sfull[slot], 0, kb * 2, nb * BN / 128);
+                    }
+                    __syncwarp();
                     if (++slot == SLOTS) slot = 0, phase ^= 1;
                 }
             }
