@@ -376,3 +376,189 @@ def test_block_norm_in_4_bits(rows, C, dt):
         v = ref.values(get(codes)[:rows, :ldc - 16], got_s[:, :nb], C)
         step = np.repeat(np.exp2(got_s[:, :nb].astype(np.float64) - 127), 32, 1)[:, :C] * 2.0
         assert (np.abs(v - get(y)) <= step + 2.0 ** -10 * np.abs(get(y))).all()
+
+
+# ------------------------------------------------------------------ together, streams, graphs, far rows
+
+def linear(rng, n, k):
+    w = blocks(rng.normal(size=(n, k)) / math.sqrt(k))
+    return w, rounded(rng.normal(size=n) * 0.1, vb.FP16)
+
+
+def mx4_space(rows, k):
+    return (torch.zeros(rows, vb.mx4_row_bytes(k), device="cuda", dtype=torch.uint8),
+            torch.zeros(vb.mx4_scale_bytes(rows, k), device="cuda", dtype=torch.uint8))
+
+
+def held(space, rows, k):
+    """The values in 64 bits that codes and scale tiles on the device stand for."""
+    nb = -(-k // 32)
+    return ref.values(get(space[0]), ref.untile_scales(get(space[1]), rows, -(-nb // 4) * 4)[:, :nb], k)
+
+
+class Block:
+    """A processor block with 4-bit Linear layers: norm -> q|k|v|self, edge attention, proj, norm with the gate,
+    mlp1 with GELU, mlp2 + residual, on one stream's buffers."""
+
+    def __init__(self, H, C, heads, seed=0):
+        rng = np.random.default_rng(seed)
+        self.H, self.C, self.heads, self.F = H, C, heads, 4 * C
+        E = 5 * H
+        ei = np.stack([rng.integers(0, H, E), rng.integers(0, H, E)]).astype(np.int64)
+        self.rp, self.src, _, self.attr = vb.build_csr(ei, rounded(rng.normal(size=(E, 3)), vb.FP16).astype(np.float32), H, H)
+        self.d_rp = torch.from_numpy(self.rp).cuda()
+        self.d_ed = torch.from_numpy(vb.pack_edges(self.src, self.attr, True)).cuda()
+        self.w4 = rounded(rng.normal(size=(4, C)) * 0.3, vb.FP16).astype(np.float32)
+        self.d_w4 = torch.from_numpy(self.w4).cuda()
+        self.lin = {n: linear(rng, o, i) for n, o, i in (("qkvs", 4 * C, C), ("proj", C, C), ("mlp1", self.F, C), ("mlp2", C, self.F))}
+        self.x = rounded(rng.normal(size=(H, C)), vb.FP16)
+        self.gate, self.scale, self.shift = (rounded(0.3 * rng.normal(size=(1, C)), vb.FP16) for _ in range(3))
+        self.w = (1 + 0.1 * rng.normal(size=C)).astype(np.float32)
+        d = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.float16)  # noqa: E731
+        self.t = {"x": put(self.x, vb.FP16), "gate": put(self.gate, vb.FP16), "scale": put(self.scale, vb.FP16),
+                  "shift": put(self.shift, vb.FP16), "w": torch.from_numpy(self.w).cuda(), "qkvs": d(H, 4 * C), "att": d(H, C),
+                  "proj": d(H, C), "x1": d(H, C), "out": d(H, C), "n1": mx4_space(H, C), "a4": mx4_space(H, C),
+                  "n2": mx4_space(H, C), "f4": mx4_space(H, self.F)}
+        self.b = {n: torch.from_numpy(v[1]).to("cuda", torch.float16) for n, v in self.lin.items()}
+
+    def run(self, stream):
+        H, C, F, t = self.H, self.C, self.F, self.t
+
+        def gemm(a, n, y, N, K, r=None, epi=0):
+            w = self.lin[n][0]
+            vb.gemm_mx4(vb.FP16, a[0], a[0].stride(0), a[1], w[0], w[0].stride(0), w[1], self.b[n], y, N, r, N, H, N, K, epi,
+                        stream=stream)
+
+        vb.block_norm(vb.FP16, H, C, t["x"], C, pre=vb.NORM_LAYER, pre_w=t["w"], scale=t["scale"], shift=t["shift"],
+                      y_codes=t["n1"][0], ldc=t["n1"][0].stride(0), y_scales=t["n1"][1], stream=stream)
+        gemm(t["n1"], "qkvs", t["qkvs"], 4 * C, C)
+        q = t["qkvs"]
+        vb.attention(vb.FP16, self.d_rp, self.d_ed, 0, H, q, 4 * C, q[:, C:], q[:, 2 * C:], 4 * C, q[:, 3 * C:], 4 * C, t["att"], C,
+                     self.d_w4, C, self.heads, C // self.heads, stream=stream)
+        vb.mx4_quantize(vb.FP16, t["att"], C, H, C, t["a4"][0], t["a4"][0].stride(0), t["a4"][1], stream=stream)
+        gemm(t["a4"], "proj", t["proj"], C, C)
+        vb.block_norm(vb.FP16, H, C, t["x"], C, h=t["proj"], ldh=C, post=vb.NORM_RMS, gate=t["gate"], out=t["x1"], ldo=C,
+                      pre=vb.NORM_LAYER, pre_w=t["w"], scale=t["scale"], shift=t["shift"], y_codes=t["n2"][0],
+                      ldc=t["n2"][0].stride(0), y_scales=t["n2"][1], stream=stream)
+        w = self.lin["mlp1"][0]
+        vb.gemm_mx4_quant(vb.FP16, t["n2"][0], t["n2"][0].stride(0), t["n2"][1], w[0], w[0].stride(0), w[1], self.b["mlp1"],
+                          t["f4"][0], t["f4"][0].stride(0), t["f4"][1], H, F, C, 1, stream=stream)
+        gemm(t["f4"], "mlp2", t["out"], C, F, t["x1"], 2)
+
+    def verify(self):
+        """Each stage against 64 bits of the stage's own inputs as the device holds them."""
+        H, C, F, t, f64 = self.H, self.C, self.F, self.t, lambda k: get(self.t[k]).astype(np.float64)
+        product_check(f64("qkvs"), held(t["n1"], H, C), self.lin["qkvs"][0][2], self.lin["qkvs"][1], None, vb.FP16, 0)
+        q = f64("qkvs")
+        att = attention(self.rp, self.src, self.attr, q, self.w4.astype(np.float64), self.heads, C)
+        assert np.abs(f64("att") - att).max() <= 2e-3 * np.abs(att).max()
+        rc, rs = ref.quantize(f64("att"))
+        assert np.array_equal(held(t["a4"], H, C), ref.values(rc, rs, C))
+        product_check(f64("proj"), held(t["a4"], H, C), self.lin["proj"][0][2], self.lin["proj"][1], None, vb.FP16, 0)
+        norm_check(f64("x1"), None, f64("x"), f64("proj"), 2, None, None, self.gate, 1.0, 0, None, None, None, None, vb.FP16)
+        for key, x in (("n1", f64("x")), ("n2", f64("x1"))):
+            y, _ = ref.norm(x, 1, self.w, None, 1e-5)
+            y = y * (1 + self.scale) + self.shift
+            n, size = ref.norm(x, 1, None, None, 1e-5)
+            e = norm_tol(x, n, size, self.w, None, vb.FP16) * (1 + np.abs(self.scale)) + 2.0 ** -21 * (np.abs(y) + np.abs(self.shift))
+            blocks_check(t[key], H, C, y, e)
+        y, err = product_exact(held(t["n2"], H, C), self.lin["mlp1"][0][2], self.lin["mlp1"][1], None, 1, False)
+        blocks_check(t["f4"], H, F, y, err)
+        product_check(f64("out"), held(t["f4"], H, F), self.lin["mlp2"][0][2], self.lin["mlp2"][1], f64("x1"), vb.FP16, 2)
+
+
+def attention(rp, src, attr, qkvs, w4, heads, C):
+    """Graph attention in 64 bits: scores and values with the edge term, + self."""
+    q, k, v, xs = (qkvs[:, i * C:(i + 1) * C] for i in range(4))
+    out, hd = xs.copy(), C // heads
+    for i in range(len(rp) - 1):
+        e = slice(rp[i], rp[i + 1])
+        if rp[i] == rp[i + 1]:
+            continue
+        term = attr[e].astype(np.float64) @ w4[:3] + w4[3]
+        kk, vv = (k[src[e]] + term).reshape(-1, heads, hd), (v[src[e]] + term).reshape(-1, heads, hd)
+        s = np.einsum("ehd,hd->eh", kk, q[i].reshape(heads, hd)) / math.sqrt(hd)
+        p = np.exp(s - s.max(0))
+        out[i] += np.einsum("eh,ehd->hd", p / p.sum(0), vv).ravel()
+    return out
+
+
+def blocks_check(space, rows, k, y, err):
+    """4-bit blocks that some number within err of y quantises to."""
+    nb = -(-k // 32)
+    sb = ref.untile_scales(get(space[1]), rows, -(-nb // 4) * 4)[:, :nb]
+    assert (ref.quantize(np.maximum(np.abs(y) - err, 0))[1] <= sb).all() and (sb <= ref.quantize(np.abs(y) + err)[1]).all()
+    v = ref.values(get(space[0]), sb, k)
+    assert (ref.round_to(y - err, sb) <= v).all() and (v <= ref.round_to(y + err, sb)).all()
+
+
+@pytest.mark.parametrize("H,C,heads", [(1, 128, 4), (300, 256, 4), (2600, 512, 8)])
+def test_block_of_4_bit_layers(H, C, heads):
+    b = Block(H, C, heads)
+    b.run(torch.cuda.current_stream().cuda_stream)
+    vb.check_device()
+    b.verify()
+
+
+def test_block_captured_replayed_and_two_at_once():
+    """A captured block replayed on new inputs, and two blocks on two streams at once, give an eager run's bits."""
+    blk = [Block(700, 256, 4, seed=i) for i in range(2)]
+    for b in blk:
+        b.run(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = [get(b.t["out"]).copy() for b in blk]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for b in blk:
+            b.t["out"].zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for b, s in zip(blk, streams):
+                b.run(s.cuda_stream)
+        torch.cuda.synchronize()
+        for b, w in zip(blk, want):
+            assert np.array_equal(get(b.t["out"]), w)
+    graphs = []
+    for b, s in zip(blk, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            b.run(s.cuda_stream)
+        graphs.append(g)
+    x = [b.t["x"].clone() for b in blk]
+    blk[0].t["x"].copy_(x[1]), blk[1].t["x"].copy_(x[0])  # other inputs
+    torch.cuda.synchronize()
+    for g, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    swapped = [get(b.t["out"]).copy() for b in blk]
+    for b, w in zip(blk, swapped):
+        b.run(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert np.array_equal(get(b.t["out"]), w) and not np.array_equal(w, want[0])
+    vb.check_device()
+
+
+def test_rows_past_32_bit_offsets():
+    """Rows whose element and byte offsets pass 2^32: a stride of 2^20 elements, 4200 rows (8.8 GB)."""
+    rows, K, N, ld = 4200, 64, 64, 1 << 20
+    rng = np.random.default_rng(4)
+    x = rounded(rng.normal(size=(rows, K)), vb.FP16)
+    big = torch.zeros(rows, ld, device="cuda", dtype=torch.float16)
+    big[:, :K] = torch.from_numpy(x).to("cuda", torch.float16)
+    codes, tiles = mx4_space(rows, K)
+    vb.mx4_quantize(vb.FP16, big, ld, rows, K, codes, K // 2, tiles)
+    rc, rs = ref.quantize(x)
+    assert np.array_equal(get(codes), rc) and np.array_equal(get(tiles), ref.tile_scales(rs))
+    W = blocks(rng.normal(size=(N, K)))
+    y = big[:, 128:]
+    vb.gemm_mx4(vb.FP16, codes, K // 2, tiles, W[0], W[0].stride(0), W[1], None, y, ld, None, 0, rows, N, K)
+    product_check(get(big[:, 128:128 + N]).astype(np.float64), ref.values(rc, rs, K), W[2], None, None, vb.FP16, 0)
+    o = big[:, 256:]
+    vb.block_norm(vb.FP16, rows, K, big, ld, pre=vb.NORM_LAYER, y=o, ldy=ld)
+    z = big[:, 384:]
+    vb.mx4_dequantize(vb.FP16, codes, K // 2, tiles, rows, K, z, ld)
+    torch.cuda.synchronize()
+    norm_check(x, get(big[:, 256:256 + K]).astype(np.float64), x, None, 0, None, None, None, 1.0, 1, None, None, None, None, vb.FP16)
+    assert np.array_equal(get(big[:, 384:384 + K]).astype(np.float64), rounded(ref.values(rc, rs, K), vb.FP16))
+    assert not big[:, 64:128].any() and not big[:, 192:256].any() and not big[:, 320:384].any() and not big[:, 448:].any()

@@ -379,20 +379,17 @@ __global__ void __launch_bounds__(kThreads, NV == 4 ? 2 : PERROW ? 4 - NV : 5 - 
                 for (int i = 0; i < NV; ++i) hr[i] = raw8(a.h + r * a.ldh, col0 + i * kLanes * 8, C, more);
             }
             F8 v[NV];
-            // (a lane's vectors of the modulation fly with the row where the registers allow)
-            constexpr bool kEarly = PERROW && (NV <= 2 || sizeof(T) == 2);
+            // PERROW: a lane's vectors of the modulation fly with the row
             Raw8<T> gr[NV], scr[NV], shr[NV];
             const int64_t gm = PERROW && a.group ? r / a.group : 0;
             const bool more_g = PERROW && a.group && gm < (a.rows - 1) / a.group;
-            auto load_gate = [&](int i) { gr[i] = raw8(a.gate + gm * a.ldgate, col0 + i * kLanes * 8, C, more_g); };
-            auto load_scale = [&](int i) { scr[i] = raw8(a.scale + gm * a.ldmod, col0 + i * kLanes * 8, C, more_g); };
-            auto load_shift = [&](int i) { shr[i] = raw8(a.shift + gm * a.ldmod, col0 + i * kLanes * 8, C, more_g); };
-            if (kEarly) {
+            if constexpr (PERROW) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    if (a.h && a.gate) load_gate(i);
-                    if (two && a.scale) load_scale(i);
-                    if (two && a.shift) load_shift(i);
+                    const int c = col0 + i * kLanes * 8;
+                    if (a.h && a.gate) gr[i] = raw8(a.gate + gm * a.ldgate, c, C, more_g);
+                    if (two && a.scale) scr[i] = raw8(a.scale + gm * a.ldmod, c, C, more_g);
+                    if (two && a.shift) shr[i] = raw8(a.shift + gm * a.ldmod, c, C, more_g);
                 }
             }
             if (!more) {
@@ -420,7 +417,6 @@ __global__ void __launch_bounds__(kThreads, NV == 4 ? 2 : PERROW ? 4 - NV : 5 - 
                     const F8 w = folded(0, i), b = folded(1, i);
                     F8 gt;
                     if (PERROW && a.gate) {
-                        if (!kEarly) load_gate(i);
                         if (!more_g) last8(gr[i], a.gate + gm * a.ldgate, c, C, more_g);
                         gt = gr[i].get();
                     }
@@ -449,14 +445,12 @@ __global__ void __launch_bounds__(kThreads, NV == 4 ? 2 : PERROW ? 4 - NV : 5 - 
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[i].p[j] = __ffma2_rn(v[i].p[j], w.p[j], b.p[j]);
                 if (PERROW && a.scale) {
-                    if (!kEarly) load_scale(i);
                     if (!more_g) last8(scr[i], a.scale + gm * a.ldmod, c, C, more_g);
                     const F8 sc = scr[i].get();
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[i].p[j] = __fmul2_rn(v[i].p[j], __fadd2_rn(sc.p[j], both(1.0f)));
                 }
                 if (PERROW && a.shift) {
-                    if (!kEarly) load_shift(i);
                     if (!more_g) last8(shr[i], a.shift + gm * a.ldmod, c, C, more_g);
                     const F8 sh = shr[i].get();
 #pragma unroll
@@ -521,13 +515,18 @@ template <class T> void block_norm(const BlockNormArgs<T>& a, cudaStream_t s) {
     const int nv = (a.C + 255) / 256;  // vectors of 8 per lane of one warp
     // a warp per row once the rows fill the SMs' warps; with fewer rows, as many warps per row as it has
     // 256-column pieces, for latency
-    // many rows: a few for each warp of a full GPU. Folding one modulation takes a CTA the time of some 50 rows
-    if (vec && nv <= 16 && a.rows >= 64 * int64_t(device_sm_count())) {
-        const bool fold = !a.group || a.group >= 1024 || (!a.gate && !a.scale && !a.shift);
+    // rows_kernel from the rows on where it is the faster one ([2000 x 1024] fp16, vectors folded: 9.7 -> 8.0 us, and
+    // [9000 x 1024] 39 -> 22; a modulation per row: [5000 x 1024] fp16 32 -> 27, but [2562 x 1000] fp32 19 -> 29, for want of
+    // registers). Folding one modulation takes a CTA the time of some 50 rows
+    const bool fold = !a.group || a.group >= 1024 || (!a.gate && !a.scale && !a.shift);
+    constexpr bool kPerRow = sizeof(T) == 2;
+    if (vec && nv <= 16 && (fold || kPerRow) && a.rows >= int64_t(fold ? 4 : 8) * device_sm_count()) {
         auto go = [&](auto n, auto lanes, auto warps) {
             constexpr int kN = decltype(n)::value, kL = decltype(lanes)::value, kW = decltype(warps)::value;
-            if (fold) launch_rows<T, kN, kL, kW, false>(a, s);
-            else launch_rows<T, kN, kL, kW, true>(a, s);
+            if constexpr (kPerRow) {
+                if (!fold) return launch_rows<T, kN, kL, kW, true>(a, s);
+            }
+            launch_rows<T, kN, kL, kW, false>(a, s);
         };
         std::integral_constant<int, 1> one;
         std::integral_constant<int, 2> n2;
