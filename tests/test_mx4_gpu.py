@@ -155,7 +155,7 @@ def product_run(A, W, bias, R, M, N, K, dt, epi, tanh=False, ld=None):
 SHAPES = [(1, 1, 1), (1, 80, 32), (1, 4096, 1024), (2, 129, 33), (3, 1000, 200), (4, 31, 64), (5, 256, 1024), (8, 70, 2100),
           (9, 1024, 4096), (17, 257, 96), (64, 512, 512), (127, 80, 184), (128, 128, 128), (129, 130, 160), (300, 1000, 1000),
           (512, 300, 320), (1000, 2048, 512), (2400, 1024, 544), (4600, 1024, 96), (5000, 1024, 1000), (20000, 800, 320),
-          (40000, 80, 256)]
+          (40000, 80, 256), (3, 500, 2100), (4, 1000, 4096), (1, 40, 5000), (2, 300, 9000), (4, 33, 8200)]
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
@@ -195,6 +195,18 @@ def test_product_nan_blocks_and_zero_rows(M):
     assert np.array_equal(np.isnan(got), nan)
     keep = np.arange(N) != 7
     assert np.array_equal(got[0, keep], bias[keep])
+
+
+@pytest.mark.parametrize("M", [2, 200])
+def test_product_of_extreme_scales(M):
+    """Scales far from 1 whose products are not: 2^p in a row of A against 2^-p in all of W, and the other way round."""
+    N, K, dt = 40, 160, vb.FP32
+    rng = np.random.default_rng(6)
+    a, w = rng.normal(size=(M, K)), rng.normal(size=(N, K))
+    for p in (60, 100, 120, -60, -100, -118):
+        A, W = blocks(a * 2.0 ** p), blocks(w * 2.0 ** -p)
+        got = product_run(A, W, None, None, M, N, K, dt, 0)
+        product_check(got, A[2], W[2], None, None, dt, 0)
 
 
 @pytest.mark.parametrize("M", [2, 200])

@@ -671,9 +671,9 @@ template <class T, int EPI, bool OUT4> void dispatch_tile(const GemmArgs<T>& a, 
 
 template <class T> void gemm(const GemmArgs<T>& a, cudaStream_t s) {
     if (a.M <= 0 || a.N <= 0) return;
-    // one or two rows, or few with a long sum that the tensor cores would form in one CTA per 64 columns ([8 x 4096] x
-    // [4096 x 1024]: 6.5 against 7.3 us; [4 x 1024] x [1024 x 4096]: 4.5 against 4.8, [8 x 1024]: 6.9 against 4.6)
-    if (!a.Yc && (a.M <= 2 || (a.M <= 8 && a.K > 2048 && a.M * a.N <= 8192))) return gemm_rows(a, s);
+    // one or two rows, or up to four with a long sum that the tensor cores would form in one CTA per 64 columns ([4 x 4096] x
+    // [4096 x 1024]: 4.7 against 7.3 us, [2 x 1024] x [1024 x 4096]: 3.4 against 4.7; [4 x 1024]: 4.5 against 4.7)
+    if (!a.Yc && (a.M <= 2 || (a.M <= kFewRows && a.K > 2048 && a.M * a.N <= 4096))) return gemm_rows(a, s);
     switch (a.epi) {
         case k::kEpiBias:
             if (a.Yc) dispatch_tile<T, k::kEpiBias, true>(a, s);

@@ -12,6 +12,8 @@
 
 namespace vb::mx4 {
 
+constexpr int kFewRows = 4;
+
 template <class T> struct GemmArgs {
     const uint8_t* A = nullptr;  // codes [M, K], lda bytes per row
     int64_t lda = 0;
@@ -32,7 +34,7 @@ template <class T> struct GemmArgs {
     bool gelu_tanh = false;
 };
 
-// Few rows of A, on the CUDA cores (Y only). Enqueues on s: no allocation, no synchronisation.
+// At most kFewRows rows of A, on the CUDA cores (Y only). Enqueues on s: no allocation, no synchronisation.
 template <class T> void gemm_rows(const GemmArgs<T>& a, cudaStream_t s);
 // Any number of rows, Y or 4-bit output: on the tensor cores, or gemm_rows. Y and R 16-byte aligned, their rows
 // a multiple of 16 bytes apart. Enqueues on s: no allocation, no synchronisation.

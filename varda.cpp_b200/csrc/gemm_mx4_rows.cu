@@ -1,5 +1,5 @@
-// The 4-bit product for few rows of A (gemm_mx4.cuh), on the CUDA cores: bound by reading the weights
-// (17/32 B per weight) and, at a row or two, by latency.
+// The 4-bit product for few rows of A (gemm_mx4.cuh), on the CUDA cores: bound by reading the weights (17/32 B per
+// weight) and, at these sizes, by latency: [1 x 1024] x [1024 x 4096] 3.0 us, of which the weights are 0.35.
 //
 // Twice an e2m1 value is a whole number (0, 1, 2, 3, 4, 6, 8, 12 and the negatives), so a block's 32
 // products are 8 dp4a on int8 values looked up from the codes, exact in 32 bits; one fp32
@@ -36,6 +36,15 @@ __device__ __forceinline__ void lookup32(uint4 u, int (&v)[8]) {
     for (int i = 0; i < 4; ++i) v[2 * i] = lookup4(w[i]), v[2 * i + 1] = lookup4(w[i] >> 16);
 }
 
+// Scale bytes from kNear to 254 - kNear (2^-95 to 2^95) need no care: a block's sum is below 2^13.
+constexpr uint32_t kNear = 32, kOne = 127;
+// d scale(sa) scale(sw) / 4 (both factors are twice their values) for any scales: the power of two in two halves.
+__device__ __noinline__ float far_product(int d, uint32_t sa, uint32_t sw) {
+    if (sa == 255u || sw == 255u) return scale_value(255u);
+    const int e = int(sa + sw) - 256, h = e >> 1;
+    return float(d) * __uint_as_float(uint32_t(max(h + 127, 1)) << 23) * __uint_as_float(uint32_t(max(e - h + 127, 1)) << 23);
+}
+
 template <class T, int MR, int WK>
 __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
     constexpr int NG = kWarps / WK;  // groups of 4 W rows per CTA
@@ -44,7 +53,6 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
     const int wk = warp % WK, gi = warp / WK;
     const int64_t nt = blockIdx.x / (32 / NG);
     const int64_t n0 = nt * 128 + (blockIdx.x % (32 / NG)) * NG + gi;  // rows n0 + 32 j
-    const int64_t m0 = int64_t(blockIdx.y) * MR;
     const int64_t nb = blocks(a.K), kt = k_tiles(a.K);
     float acc[kRowsW][MR];
 #pragma unroll
@@ -53,22 +61,23 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
         for (int m = 0; m < MR; ++m) acc[j][m] = 0.0f;
     for (int64_t b = wk * 32 + lane; b < nb; b += WK * 32) {
         uint4 w[kRowsW];
-        float fw[kRowsW];
+        uint32_t sw[kRowsW], sa[MR];
+        bool far = false;  // a scale whose product with a block's sum may leave fp32 before the other scale brings it back
 #pragma unroll
         for (int j = 0; j < kRowsW; ++j) {
             const int64_t n = n0 + 32 * j;
             const bool in = n < a.N;
             w[j] = in ? __ldg(reinterpret_cast<const uint4*>(a.W + n * a.ldw) + b) : make_uint4(0, 0, 0, 0);
-            // both factors are twice their values: 1/4 here
-            fw[j] = in ? 0.25f * scale_value(__ldg(a.sW + scale_at(n, b, kt))) : 0.0f;
+            sw[j] = in ? __ldg(a.sW + scale_at(n, b, kt)) : kOne;
+            far |= sw[j] - kNear > 254u - 2 * kNear;
         }
         int av[MR][8];
-        float fa[MR];
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
-            const bool in = m0 + m < a.M;
-            const uint4 u = in ? __ldg(reinterpret_cast<const uint4*>(a.A + (m0 + m) * a.lda) + b) : make_uint4(0, 0, 0, 0);
-            fa[m] = in ? scale_value(__ldg(a.sA + scale_at(m0 + m, b, kt))) : 0.0f;
+            const bool in = m < a.M;
+            const uint4 u = in ? __ldg(reinterpret_cast<const uint4*>(a.A + m * a.lda) + b) : make_uint4(0, 0, 0, 0);
+            sa[m] = in ? __ldg(a.sA + scale_at(m, b, kt)) : kOne;
+            far |= sa[m] - kNear > 254u - 2 * kNear;
             lookup32(u, av[m]);
         }
 #pragma unroll
@@ -80,7 +89,8 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
                 int d = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d = __dp4a(av[m][i], wv[i], d);
-                acc[j][m] = __fmaf_rn(float(d) * fa[m], fw[j], acc[j][m]);
+                if (!far) acc[j][m] = __fmaf_rn(float(d) * scale_value(sa[m]), 0.25f * scale_value(sw[j]), acc[j][m]);
+                else acc[j][m] += far_product(d, sa[m], sw[j]);
             }
         }
     }
@@ -93,7 +103,7 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
         }
     __syncthreads();
     if (wk != 0 || lane >= kRowsW * MR) return;
-    const int64_t n = n0 + 32 * (lane % kRowsW), m = m0 + lane / kRowsW;
+    const int64_t n = n0 + 32 * (lane % kRowsW), m = lane / kRowsW;
     if (n >= a.N || m >= a.M) return;
     float y = 0.0f;
 #pragma unroll
@@ -105,9 +115,9 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
 }
 
 template <class T, int MR, int WK> void launch(const GemmArgs<T>& a, cudaStream_t s) {
-    const int64_t gx = (a.N + 127) / 128 * (32 / (kWarps / WK)), gy = (a.M + MR - 1) / MR;
-    if (gx > INT32_MAX || gy > 65535) fail(kUnsupported, "gemm_mx4: too many rows for the few-row kernel");
-    rows_kernel<T, MR, WK><<<dim3(unsigned(gx), unsigned(gy)), 32 * kWarps, 0, s>>>(a);
+    const int64_t grid = (a.N + 127) / 128 * (32 / (kWarps / WK));
+    if (grid > INT32_MAX) fail(kUnsupported, "gemm_mx4: too many columns for one launch");
+    rows_kernel<T, MR, WK><<<unsigned(grid), 32 * kWarps, 0, s>>>(a);
     VB_LAUNCH();
 }
 
@@ -124,10 +134,10 @@ template <class T, int MR> void dispatch_k(const GemmArgs<T>& a, cudaStream_t s)
 
 template <class T> void gemm_rows(const GemmArgs<T>& a, cudaStream_t s) {
     if (a.M <= 0 || a.N <= 0) return;
+    if (a.M > kFewRows) fail(kInvalidArgument, "gemm_mx4: too many rows for the few-row kernel");
     if (a.M == 1) dispatch_k<T, 1>(a, s);
     else if (a.M == 2) dispatch_k<T, 2>(a, s);
-    else if (a.M <= 4) dispatch_k<T, 4>(a, s);
-    else dispatch_k<T, 8>(a, s);
+    else dispatch_k<T, kFewRows>(a, s);
 }
 
 template void gemm_rows<float>(const GemmArgs<float>&, cudaStream_t);
