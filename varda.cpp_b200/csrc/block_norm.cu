@@ -264,12 +264,19 @@ __device__ __forceinline__ void cut(F8& f, int c, int C) {
     }
 }
 
+// CTAs per SM that the registers are cut for. More rows in flight are worth some spilling at fp16 ([189809 x 1024] 299 us
+// with 2, 273 with 3; 512 columns 154 with 3, 142 with 4), not at fp32 (1024 columns 553 with 2, 680 with 3).
+template <class T> constexpr int rows_ctas(int nv, bool perrow) {
+    if (nv == 4) return sizeof(T) == 2 && !perrow ? 3 : 2;
+    return (perrow ? 4 : sizeof(T) == 2 ? 6 : 5) - nv;
+}
+
 // Many rows: CTA b takes rows [b per, (b + 1) per), LPR lanes of a warp or WPR warps per row, NV vectors of 8
 // columns per lane. Shared memory: four vectors, A1, B1, A2, B2 of the modulation's rows (the range is cut where
 // that changes), or with PERROW (a modulation per row or few rows, loaded with the row) the norms' weights and
 // biases; each as the first and the second four of the lanes' eights, so that a warp reads 512 consecutive bytes.
 template <class T, int NV, int LPR, int WPR, bool PERROW>
-__global__ void __launch_bounds__(kThreads, NV == 4 ? 2 : PERROW ? 4 - NV : 5 - NV)
+__global__ void __launch_bounds__(kThreads, rows_ctas<T>(NV, PERROW))
     rows_kernel(BlockNormArgs<T> a, int64_t ktiles, int64_t per) {
     constexpr int kLanes = LPR * WPR, kRows = kThreads / kLanes;  // lanes per row, rows at a time
     constexpr int kVecs = NV * kLanes;                             // vectors of 8 columns per row
