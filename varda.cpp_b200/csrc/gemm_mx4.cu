@@ -3,14 +3,17 @@
 //
 // Persistent and warp-specialised: one 768-thread CTA per SM, or clusters of two with cta_group::2 computing
 // 256-row tiles together (each CTA loads its 128 rows of A and half of the W tile).
-//   warp 0 (one lane)   TMA producer: codes of A [128 x 128 bytes = 256 columns of K] and of W, 128-byte
+//   warp 0              TMA producer: codes of A [128 x 128 bytes = 256 columns of K] and of W, 128-byte
 //                       swizzle, into a ring of kStages.
-//   warp 2 (one lane)   TMA producer of their scale tiles (512 bytes per 128 rows and 128 columns, stored in
+//   warp 2              TMA producer of their scale tiles (512 bytes per 128 rows and 128 columns, stored in
 //                       the order in which tensor memory holds them) into a ring of kSlots.
 //   warps 4-7           scales from shared into tensor memory, each warp its lane quarter's copy, into the buffer
 //                       of the stage (as many as stages). (tcgen05.cp does the same from the MMA thread, but
-//                       the tensor pipe runs it between the MMAs: 57 cycles per 512 bytes, 2970 TFLOP/s at most.)
-//   warp 1 (one lane)   MMA issuer: four MMAs of K = 64 per stage; in a last stage that K cuts, only those it needs.
+//                       the tensor pipe runs it between the MMAs, some 57 cycles for 512 bytes: [189809 x 4096] x
+//                       [4096 x 1024] took 470 us with it, 365 with these warps.)
+//   warp 1              MMA issuer: four MMAs of K = 64 per stage; in a last stage that K cuts, only those it needs.
+//                       (These three warps run their loops whole and issue through one elected lane: the operands
+//                       are then uniform values. 3-5% on the long sums against one lane in a branch.)
 //   warps 8-23          epilogue: a warp takes 32 rows and a quarter of the tile's columns into registers at
 //                       once and hands the accumulator back, then bias / GELU / residual in fp32, one rounding
 //                       and a TMA store from swizzled shared memory (the residual came by TMA into the same
@@ -18,7 +21,14 @@
 //                       block's scale is the maximum of the lane's registers.
 // Tensor memory at BN = 256: two accumulators would fill all 512 columns, but the scales need some. So the
 // second accumulator starts at column 128, over half of the first; since the epilogue reads all columns
-// at once, the next tile's MMAs start a few hundred cycles after the last one's.
+// at once, the next tile's MMAs start some 1300 cycles after the last one's end.
+//
+// What bounds it: [189809 x 1024] x [1024 x 4096] 442 us with a bias (1.55 GB of output, which alone takes 390 us to fill),
+// 545 with GELU (the epilogue: instruction issue 60%, special functions 38%, the fp32 pipe 42%), and
+// [189809 x 4096] x [4096 x 1024] + residual 365 us = 4360 TFLOP/s (tensor pipe 58%; the loads alone take 320 us, some
+// 10 TB/s from L2); run for seconds all of them are held by the 1 kW power limit (1.4 GHz: 420 us). Tried and dropped:
+// 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us with a bias), the same with A's
+// rows kept in shared memory (533), plain stores instead of TMA stores (517).
 //
 // Every wait is bounded as in gemm_tc.cu: on timeout a CTA sets the device error flag, stops issuing, waits for
 // its own copies and MMAs in flight, frees its tensor memory and returns.
@@ -111,7 +121,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 
 // Arrival on a barrier of the pair that tells of tensor memory read or written: tcgen05.fence orders that, and
 // no other memory goes with it. (A release at cluster scope waits about 1000 cycles for the thread's other
-// writes: 1000 us instead of 330 on [189809 x 4096] x [4096 x 1024].)
+// writes: 1000 us instead of 450 on [189809 x 4096] x [4096 x 1024] then.)
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -157,8 +167,8 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 // GELU in fp32 with one special-function operation: x Phi(x) = max(x, 0) - z Phi(-z), z = |x|, and
 // Phi(-z) = 2^P(z) with P a polynomial fitted to log2 Phi(-z) on [0, 5.6] (weighted least squares towards the
 // smallest largest error of z Phi(-z)): |error| <= 3e-7, at most 5e-7 |x|. Past 5.6, z Phi(-z) stays at its
-// 6e-8. (The two-operation form of gemm_tc.cu is bound by the special-function units here: 16 a clock and
-// SM make 345 us on [189809 x 1024] x [1024 x 4096].)
+// 6e-8. (gemm_tc.cu's form takes two: at 16 a clock and SM they alone make 345 us on [189809 x 1024] x [1024 x 4096].
+// Scalar instead of packed operations: 650 us there, against 587 then.)
 __device__ __forceinline__ float2 gelu2(float2 x) {
     const float2 n = make_float2(fmaxf(-fabsf(x.x), -5.6f), fmaxf(-fabsf(x.y), -5.6f));
     float2 p = __ffma2_rn(n, make_float2(3.26786503e-05f, 3.26786503e-05f), make_float2(7.58978247e-04f, 7.58978247e-04f));

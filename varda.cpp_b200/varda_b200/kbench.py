@@ -8,7 +8,8 @@ hidden graph of C1 (189,809 nodes, ~2.6M directed multi-scale edges in CSR by de
 16 heads of 64, 3-dim edge attributes uniform[0,1], node features N(0,1), seeded. q, k, v and x_r
 are column slices of one [H, 4C] buffer as in the processor block. Reported: ms per launch, and the
 compulsory bytes per launch (q, x_r, out per destination, k and v per source, 16 bytes per edge,
-row_ptr, edge weights) divided by it.
+row_ptr, edge weights) divided by it. `mx4`: quantising A, reading it back, and the 4-bit product (--quant: with
+4-bit output); `norm`: the gated block norm (LayerNorm of h, gate, residual, LayerNorm, modulation).
 """
 from __future__ import annotations
 
@@ -131,6 +132,70 @@ def attention(a):
               flush=True)
 
 
+def _report(name, ms, byt, flop=0.0, **more):
+    gbs = byt / ms / 1e6
+    d = {"kernel": name, **more, "ms": round(ms, 4), "bytes": byt, "gbs": round(gbs, 1),
+         "frac_of_hbm": round(gbs / _peaks()["hbm_gbs"], 4)}
+    if flop:
+        d["tflops"] = round(flop / ms / 1e9, 1)
+    print(json.dumps(d), flush=True)
+
+
+def mx4(a):
+    import torch
+    dt, T, z = (vb.FP16, torch.float16, 2) if a.dtype == "fp16" else (vb.FP32, torch.float32, 4)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    s = torch.cuda.current_stream().cuda_stream
+    u8 = lambda *n: torch.empty(*n, device="cuda", dtype=torch.uint8)  # noqa: E731
+
+    def blocks(x):
+        rows, k = x.shape
+        c, sc = u8(rows, vb.mx4_row_bytes(k)), u8(vb.mx4_scale_bytes(rows, k))
+        return c, sc, lambda: vb.mx4_quantize(dt, x, k, rows, k, c, c.stride(0), sc, stream=s)
+
+    x = torch.randn(a.M, a.K, device="cuda", generator=g).to(T)
+    A, sA, quant = blocks(x)
+    W, sW, quant_w = blocks((torch.randn(a.N, a.K, device="cuda", generator=g) / math.sqrt(a.K)).to(T))
+    quant_w()
+    shape = {"M": a.M, "K": a.K, "dtype": a.dtype}
+    held = lambda rows, k: rows * -(-k // 32) * 17.0  # noqa: E731
+    _report("mx4_quantize", time_launches(quant, a.iters, a.warmup), z * x.numel() + held(a.M, a.K), **shape)
+    _report("mx4_dequantize", time_launches(lambda: vb.mx4_dequantize(dt, A, A.stride(0), sA, a.M, a.K, x, a.K, stream=s),
+                                            a.iters, a.warmup), z * x.numel() + held(a.M, a.K), **shape)
+    b = torch.randn(a.N, device="cuda", generator=g).to(T)
+    ld = -(-a.N // 8) * 8
+    byt = held(a.M, a.K) + held(a.N, a.K) + z * a.N
+    if a.quant:
+        Y, sY = u8(a.M, vb.mx4_row_bytes(a.N)), u8(vb.mx4_scale_bytes(a.M, a.N))
+        fn = lambda: vb.gemm_mx4_quant(dt, A, A.stride(0), sA, W, W.stride(0), sW, b, Y, Y.stride(0), sY, a.M, a.N,  # noqa: E731
+                                       a.K, a.epi, stream=s)
+        byt += held(a.M, a.N)
+    else:
+        Y = torch.empty(a.M, ld, device="cuda", dtype=T)
+        R = torch.randn(a.M, ld, device="cuda", generator=g).to(T) if a.epi == 2 else None
+        fn = lambda: vb.gemm_mx4(dt, A, A.stride(0), sA, W, W.stride(0), sW, b, Y, ld, R, ld, a.M, a.N, a.K, a.epi,  # noqa: E731
+                                 stream=s)
+        byt += z * a.M * a.N * (2 if a.epi == 2 else 1)
+    _report("gemm_mx4_quant" if a.quant else "gemm_mx4", time_launches(fn, a.iters, a.warmup), byt, 2.0 * a.M * a.N * a.K,
+            N=a.N, epi=a.epi, **shape)
+
+
+def norm(a):
+    import torch
+    dt, T, z = (vb.FP16, torch.float16, 2) if a.dtype == "fp16" else (vb.FP32, torch.float32, 4)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ld, groups = -(-a.C // 8) * 8, -(-a.rows // a.group) if a.group else 1
+    t = lambda n: torch.randn(n, ld, device="cuda", generator=g).to(T)  # noqa: E731
+    x, h, gate, sc, sh, out, y = t(a.rows), t(a.rows), t(groups), t(groups), t(groups), t(a.rows), t(a.rows)
+    w, b = (torch.randn(a.C, device="cuda", generator=g) for _ in range(2))
+    s = torch.cuda.current_stream().cuda_stream
+    fn = lambda: vb.block_norm(dt, a.rows, a.C, x, ld, h=h, ldh=ld, post=vb.NORM_LAYER, post_w=w, post_b=b, gate=gate,  # noqa: E731
+                               ldgate=ld, out=out, ldo=ld, pre=vb.NORM_LAYER, pre_w=w, pre_b=b, scale=sc, shift=sh, ldmod=ld,
+                               rows_per_group=a.group, y=y, ldy=ld, stream=s)
+    _report("block_norm", time_launches(fn, a.iters, a.warmup), z * a.C * (4.0 * a.rows + 3.0 * groups), rows=a.rows, C=a.C,
+            group=a.group, dtype=a.dtype)
+
+
 def main():
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -152,8 +217,22 @@ def main():
     t.add_argument("--impl", default="tc", help="comma-separated: tc, tiled, gather")
     t.add_argument("--iters", type=int, default=20)
     t.add_argument("--warmup", type=int, default=3)
+    m = sub.add_parser("mx4")
+    m.add_argument("--M", type=int, default=189809)
+    m.add_argument("--N", type=int, default=4096)
+    m.add_argument("--K", type=int, default=1024)
+    m.add_argument("--epi", type=int, default=0)
+    m.add_argument("--quant", action="store_true", help="4-bit output (epilogue 0 or 1)")
+    n = sub.add_parser("norm")
+    n.add_argument("--rows", type=int, default=189809)
+    n.add_argument("--C", type=int, default=1024)
+    n.add_argument("--group", type=int, default=0, help="rows per modulation row (0: one for all)")
+    for p in (m, n):
+        p.add_argument("--dtype", default="fp16", choices=["fp16", "fp32"])
+        p.add_argument("--iters", type=int, default=20)
+        p.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args()
-    {"gemm": gemm, "attention": attention}[a.cmd](a)
+    {"gemm": gemm, "attention": attention, "mx4": mx4, "norm": norm}[a.cmd](a)
 
 
 if __name__ == "__main__":
