@@ -292,7 +292,8 @@ int vb_add_layernorm(int dtype, const void* a, const void* r, void* out1, const 
  *           bytes, block tiles of the same rows side by side): byte (row % 32) * 16 + (row % 128) / 32 * 4 +
  *           block % 4 of tile (row / 128, block / 4). The bytes of a row's blocks past ceil(K / 32) must not
  *           be 255 (the functions here write 0); those of rows past the last are not used.
- * The same dtype, stream and error rules as above; nothing is allocated; calls may be captured. */
+ * The same dtype, stream and error rules as above; nothing is allocated and there is no workspace, so calls may
+ * be captured and may overlap. Outputs must not overlap inputs but where that is said. */
 int64_t vb_mx4_row_bytes(int64_t K);
 int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K);
 

@@ -155,7 +155,8 @@ def product_run(A, W, bias, R, M, N, K, dt, epi, tanh=False, ld=None):
 SHAPES = [(1, 1, 1), (1, 80, 32), (1, 4096, 1024), (2, 129, 33), (3, 1000, 200), (4, 31, 64), (5, 256, 1024), (8, 70, 2100),
           (9, 1024, 4096), (17, 257, 96), (64, 512, 512), (127, 80, 184), (128, 128, 128), (129, 130, 160), (300, 1000, 1000),
           (512, 300, 320), (1000, 2048, 512), (2400, 1024, 544), (4600, 1024, 96), (5000, 1024, 1000), (20000, 800, 320),
-          (40000, 80, 256), (3, 500, 2100), (4, 1000, 4096), (1, 40, 5000), (2, 300, 9000), (4, 33, 8200)]
+          (40000, 80, 256), (3, 500, 2100), (4, 1000, 4096), (1, 40, 5000), (2, 300, 9000), (4, 33, 8200), (129, 1, 64),
+          (130, 7, 33), (5, 3, 1)]
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
@@ -574,3 +575,24 @@ def test_rows_past_32_bit_offsets():
     norm_check(x, get(big[:, 256:256 + K]).astype(np.float64), x, None, 0, None, None, None, 1.0, 1, None, None, None, None, vb.FP16)
     assert np.array_equal(get(big[:, 384:384 + K]).astype(np.float64), rounded(ref.values(rc, rs, K), vb.FP16))
     assert not big[:, 64:128].any() and not big[:, 192:256].any() and not big[:, 320:384].any() and not big[:, 448:].any()
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are made inside a stream capture: nothing in them is forbidden there."""
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = %r
+import numpy as np, torch, varda_b200 as vb
+import test_mx4_gpu as t
+b = t.Block(2600, 512, 8)
+s = torch.cuda.Stream(); torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    b.run(s.cuda_stream)
+with torch.cuda.stream(s):
+    g.replay()
+torch.cuda.synchronize(); vb.check_device(); b.verify(); print("verified")
+""" % [p for p in sys.path if p]
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "verified" in r.stdout, r.stderr[-2000:]

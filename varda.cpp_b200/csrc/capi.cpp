@@ -73,7 +73,6 @@ void need(const void* p, const char* what) {
 // The kernels' device-side timeout flags (read and cleared; synchronises the device).
 void device_errors() {
     if (vb::tc::take_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the tensor-core GEMM");
-    if (vb::mx4::take_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the 4-bit GEMM");
     if (vb::k::take_attention_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the attention");
 }
 
@@ -222,7 +221,11 @@ size_t vb_activation_bytes(const vb_model* m) { return m ? m->m->activation_byte
 int64_t vb_decoder_chunk_rows(const vb_model* m) { return m ? m->m->decoder_chunk_rows() : 0; }
 
 int vb_check_device(void) {
-    return guard([&] { device_errors(); });
+    return guard([&] {
+        const int mx4 = vb::mx4::take_error();  // (the engine has none of these GEMMs)
+        device_errors();
+        if (mx4) vb::fail(vb::kTimeout, "a device-side wait timed out in the 4-bit GEMM");
+    });
 }
 
 int64_t vb_shard_plan(const char* path, int world, int rank, char* buf, size_t len) {

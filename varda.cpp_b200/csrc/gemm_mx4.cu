@@ -63,8 +63,6 @@ __device__ int g_error = 0;
 
 struct Params {
     const void* bias;
-    const void* R;
-    int64_t ldr;
     void* Y;
     int64_t ldy;
     uint8_t* Yc;
@@ -642,7 +640,7 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
         ty = rows_map(a.Y, a.M, a.N, a.ldy, L::kSW);
         if (EPI == k::kEpiResidual) tr = rows_map(a.R, a.M, a.N, a.ldr, L::kSW);
     }
-    const Params p{a.bias, a.R, a.ldr, a.Y, a.ldy, a.Yc, a.ldyc, a.Ys, k_tiles(a.N), int(a.M), int(a.N), int((a.K + 63) / 64),
+    const Params p{a.bias, a.Y, a.ldy, a.Yc, a.ldyc, a.Ys, k_tiles(a.N), int(a.M), int(a.N), int((a.K + 63) / 64),
                    a.gelu_tanh ? 1 : 0};
     constexpr int UM = PAIR ? 2 * BM : BM;
     const int64_t tiles = ((a.M + UM - 1) / UM) * ((a.N + BN - 1) / BN);
