@@ -1,7 +1,5 @@
 """The 4-bit Linear layers and the gated block norm on the CPU: sizes, and every refusal (made on the host,
 before anything is launched)."""
-import ctypes
-
 import numpy as np
 import pytest
 
@@ -88,7 +86,7 @@ def test_block_norm_refuses_wide_rows_and_no_arguments():
     wide = dict(C=16385, ldx=16385, ldh=16385, ldgate=16385, ldo=16385, ldmod=16385, ldy=16385)
     refused(lambda: vb.block_norm(**{**NORM, **wide}), code=4)
     assert vb.lib.vb_block_norm(vb.FP16, None, None) == 1
-    assert ctypes.sizeof(vb.BlockNormArgs) == 23 * 8 + 16
+    assert vb.BLOCK_NORM_ARGS.size == 23 * 8 + 16  # which the library checks of its struct
 
 
 def test_nothing_to_do_is_no_error():

@@ -786,6 +786,8 @@ int vb_gemm_mx4_quant(int dtype, const void* A, int64_t lda, const void* sA, con
     });
 }
 
+static_assert(sizeof(vb_block_norm_args) == 23 * 8 + 16, "the binding packs the arguments without padding");
+
 int vb_block_norm(int dtype, const vb_block_norm_args* p, void* stream) {
     return guard([&] {
         dtype_size(dtype);
