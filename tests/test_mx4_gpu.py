@@ -118,10 +118,17 @@ def product_case(M, N, K, dt, seed=0):
     return blocks(A), blocks(W), rounded(rng.normal(size=N), dt), rounded(rng.normal(size=(M, N)), dt)
 
 
+def matmul(a, w):
+    """a w^T in 64 bits, by the device's 64-bit matrix product (small ones here)."""
+    if len(a) * len(w) * a.shape[1] < 10 ** 9:
+        return a @ w.T
+    return (torch.from_numpy(a).cuda() @ torch.from_numpy(w).cuda().t()).cpu().numpy()
+
+
 def product_exact(a, w, bias, R, epi, tanh):
     """(the result in 64 bits, the bound of an fp32 evaluation's error)."""
     K = a.shape[1]
-    y, mag = a @ w.T, np.abs(a) @ np.abs(w).T
+    y, mag = matmul(a, w), matmul(np.abs(a), np.abs(w))
     if bias is not None:
         y, mag = y + bias, mag + np.abs(bias)
     err = (K + 8) * 2.0 ** -23 * mag
@@ -156,7 +163,7 @@ SHAPES = [(1, 1, 1), (1, 80, 32), (1, 4096, 1024), (2, 129, 33), (3, 1000, 200),
           (9, 1024, 4096), (17, 257, 96), (64, 512, 512), (127, 80, 184), (128, 128, 128), (129, 130, 160), (300, 1000, 1000),
           (512, 300, 320), (1000, 2048, 512), (2400, 1024, 544), (4600, 1024, 96), (5000, 1024, 1000), (20000, 800, 320),
           (40000, 80, 256), (3, 500, 2100), (4, 1000, 4096), (1, 40, 5000), (2, 300, 9000), (4, 33, 8200), (129, 1, 64),
-          (130, 7, 33), (5, 3, 1)]
+          (130, 7, 33), (5, 3, 1), (40000, 1000, 96), (20000, 1000, 1100), (20001, 1001, 1100), (20000, 998, 1100)]
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
@@ -229,7 +236,8 @@ def test_product_residual_in_place_and_strided_codes(M):
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 64, 64), (3, 70, 200), (7, 192, 96), (129, 100, 64), (300, 1000, 320),
-                                   (2400, 1000, 224), (5000, 1024, 96), (20000, 800, 160)])
+                                   (2400, 1000, 224), (5000, 1024, 96), (20000, 800, 160), (40000, 1000, 96),
+                                   (20001, 1000, 1100)])
 def test_product_in_4_bits(M, N, K, dt):
     """The output blocks: scale and values are those of some number within the fp32 error of the exact one."""
     A, W, bias, _ = product_case(M, N, K, dt, 1)

@@ -2,7 +2,7 @@
 // multiplies 64 e2m1 values of a row and column at a time, each block of 32 with its two scales, into fp32.
 //
 // Persistent and warp-specialised: one 768-thread CTA per SM, or clusters of two with cta_group::2 computing
-// 256-row tiles together (each CTA loads its 128 rows of A and half of the W tile).
+// 256 x 256 tiles together (each CTA loads its 128 rows of A and half of the W tile).
 //   warp 0              TMA producer: codes of A [128 x 128 bytes = 256 columns of K] and of W, 128-byte
 //                       swizzle, into a ring of kStages.
 //   warp 2              TMA producer of their scale tiles (512 bytes per 128 rows and 128 columns, stored in
@@ -668,11 +668,15 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
 template <class T, int EPI, bool OUT4> void dispatch_tile(const GemmArgs<T>& a, cudaStream_t s) {
     auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
     const int64_t sms = device_sm_count();
-    // the largest tile that still gives every SM (pair) one, and no wider than N ([40321 x 1024] x [1024 x 80]: 11 us,
-    // with 256-column tiles 17)
-    if (a.N > 128 && tiles(256, 256) >= sms / 2) launch<T, 256, true, EPI, OUT4>(a, s);
-    else if (tiles(128, 128) >= sms) launch<T, 128, false, EPI, OUT4>(a, s);
-    else launch<T, 64, false, EPI, OUT4>(a, s);
+    // 64 columns where that gives an SM no second tile ([5000 x 512] x [512 x 256]: 5.3 us, with 128 columns 4.9 where it
+    // does, at 700 rows 4.4 against 4.9). The pairs' 256 columns once they have several each, sooner for long sums, whose
+    // loads they halve ([20000 x 512] x [512 x 1024], 4 each: 14.5 against 12.6; [100000 x 512] x [512 x 2048], 42: 87
+    // against 92; [60000 x 2048] x [2048 x 512] with GELU, 6: 40 against 44), but not for fp32 output after short ones, which the
+    // stores bound ([100000 x 512] x [512 x 2048]: 174 against 139)
+    const bool stores = sizeof(T) == 4 && !OUT4 && a.K <= 512;
+    if (tiles(128, 64) <= sms) launch<T, 64, false, EPI, OUT4>(a, s);
+    else if (a.N > 128 && !stores && tiles(256, 256) >= (a.K > 1024 ? 4 : 8) * (sms / 2)) launch<T, 256, true, EPI, OUT4>(a, s);
+    else launch<T, 128, false, EPI, OUT4>(a, s);
 }
 
 }  // namespace
