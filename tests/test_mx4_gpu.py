@@ -205,6 +205,30 @@ def test_product_nan_blocks_and_zero_rows(M):
     assert np.array_equal(got[0, keep], bias[keep])
 
 
+@pytest.mark.parametrize("M,N,K", [(2, 70, 64), (5, 100, 96), (300, 1000, 1100), (20000, 1001, 1100)])
+def test_product_ignores_the_scale_bytes_of_absent_rows(M, N, K):
+    """Whatever the last tiles hold for rows past M and N: the same bits, in values and in 4-bit blocks."""
+    A, W, bias, R = product_case(M, N, K, vb.FP16, 4)
+    ld, ldc, z = (N + 7) // 8 * 8, vb.mx4_row_bytes(N), vb.mx4_scale_bytes(M, N)
+    b = torch.from_numpy(bias).to("cuda", torch.float16)
+    present = np.ones((M, -(-N // 32)), np.uint8)
+    outs = []
+    for byte in (0, 255):
+        sc = []
+        for t, rows in ((A[1], M), (W[1], N)):
+            absent = ref.tile_scales(np.ones((rows, 4 * -(-K // 128)), np.uint8)) == 0
+            t = t.clone()
+            t[torch.from_numpy(absent).cuda()] = byte
+            sc.append(t)
+        y = torch.zeros(M, ld, device="cuda", dtype=torch.float16)
+        vb.gemm_mx4(vb.FP16, A[0], A[0].stride(0), sc[0], W[0], W[0].stride(0), sc[1], b, y, ld, None, 0, M, N, K, 0)
+        codes, tiles = torch.zeros(M, ldc, device="cuda", dtype=torch.uint8), torch.zeros(z, device="cuda", dtype=torch.uint8)
+        vb.gemm_mx4_quant(vb.FP16, A[0], A[0].stride(0), sc[0], W[0], W[0].stride(0), sc[1], b, codes, ldc, tiles, M, N, K, 1)
+        vb.check_device()
+        outs.append((get(y), get(codes), get(tiles)[ref.tile_scales(present) == 1]))
+    assert all(np.array_equal(p, q) for p, q in zip(*outs))
+
+
 @pytest.mark.parametrize("M", [2, 200])
 def test_product_of_extreme_scales(M):
     """Scales far from 1 whose products are not: 2^p in a row of A against 2^-p in all of W, and the other way round."""
