@@ -341,7 +341,8 @@ def norm_run(x, h, post, pw, pb, g, rs, pre, w, b, sc, sh, group, dt, ld=None, s
 
 
 NORM_SHAPES = [(1, 1), (2, 7), (9, 8), (5, 100), (3, 256), (1, 1024), (33, 1000), (7, 2048), (3, 2056), (2, 5000), (2, 16384),
-               (1300, 264), (1200, 1024), (1201, 2000), (1199, 517)]
+               (1300, 264), (1200, 1024), (1201, 2000), (1199, 517), (1300, 700), (1250, 1404), (1205, 2800), (1300, 4104),
+               (1190, 6004), (1195, 8192), (1189, 8200), (1204, 1404), (1204, 2800), (1300, 5000), (1300, 8096)]
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
@@ -396,7 +397,8 @@ def test_block_norm_constant_rows_and_not_finite():
 
 
 @pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
-@pytest.mark.parametrize("rows,C", [(1, 32), (3, 1000), (130, 96), (40, 1), (1300, 1024), (1250, 100), (5, 4100)])
+@pytest.mark.parametrize("rows,C", [(1, 32), (3, 1000), (130, 96), (40, 1), (1300, 1024), (1250, 100), (5, 4100), (1200, 744),
+                                    (1300, 5000), (1190, 8100)])
 def test_block_norm_in_4_bits(rows, C, dt):
     """The 4-bit output is the quantised fp32 y: with fp32 storage, the same bits as quantising the y it stores."""
     rng = np.random.default_rng(rows + C)

@@ -114,9 +114,11 @@ __device__ __forceinline__ void store_blocks(const BlockNormArgs<T>& a, int64_t 
     if (live && (c & 127) == 0 && c < C) *reinterpret_cast<uint32_t*>(a.ys + mx4::scale_at(r, c / mx4::kBlock, ktiles)) = w;
 }
 
-// WPR warps per row, NV vectors of 8 columns per thread.
-template <class T, int NV, int WPR, bool VEC>
-__global__ void __launch_bounds__(kThreads) few_kernel(BlockNormArgs<T> a, int64_t ktiles) {
+// WPR warps per row, NV vectors of 8 columns per thread. EARLY: the pre-norm's modulation is loaded with the row, for
+// latency; otherwise it is only fetched into L2, which leaves registers for two more CTAs per SM ([2562 x 1000] fp32, a
+// modulation per row: 18.8 us early, 17.3 late, [20000 x 1000] 108 and 99; [1 x 1024] fp16 4.3 and 4.7).
+template <class T, int NV, int WPR, bool VEC, bool EARLY>
+__global__ void __launch_bounds__(kThreads, NV == 8 ? 1 : NV == 4 ? 2 : NV == 2 || EARLY ? 4 : 6) few_kernel(BlockNormArgs<T> a, int64_t ktiles) {
     __shared__ float red[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = int64_t(blockIdx.x) * (kWarps / WPR) + warp / WPR;
@@ -125,8 +127,6 @@ __global__ void __launch_bounds__(kThreads) few_kernel(BlockNormArgs<T> a, int64
     const int C = live ? a.C : 0;  // (a row past the end has no columns, but takes part in the sums)
     const int c0 = ((warp % WPR) * 32 + lane) * 8;
     const int64_t g = a.group ? r / a.group : 0;
-    // one vector per thread: the modulation's loads fly with the row's
-    constexpr bool kEarly = NV == 1;
     float x[NV][8], h[NV][8], gt[8], sc[8], sh[8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) load8<T, VEC>(a.x + r * a.ldx, c0 + i * WPR * 256, C, x[i]);
@@ -134,16 +134,21 @@ __global__ void __launch_bounds__(kThreads) few_kernel(BlockNormArgs<T> a, int64
 #pragma unroll
         for (int i = 0; i < NV; ++i) load8<T, VEC>(a.h + r * a.ldh, c0 + i * WPR * 256, C, h[i]);
     }
-    if (kEarly && a.h && a.gate) load8<T, VEC>(a.gate + g * a.ldgate, c0, C, gt);
-    if (kEarly && a.scale) load8<T, VEC>(a.scale + g * a.ldmod, c0, C, sc);
-    if (kEarly && a.shift) load8<T, VEC>(a.shift + g * a.ldmod, c0, C, sh);
+    if (NV == 1 && a.h && a.gate) load8<T, VEC>(a.gate + g * a.ldgate, c0, C, gt);
+    if constexpr (EARLY) {
+        if (a.scale) load8<T, VEC>(a.scale + g * a.ldmod, c0, C, sc);
+        if (a.shift) load8<T, VEC>(a.shift + g * a.ldmod, c0, C, sh);
+    } else if (NV == 1 && c0 < C) {
+        if (a.scale) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.scale + g * a.ldmod + c0));
+        if (a.shift) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.shift + g * a.ldmod + c0));
+    }
     if (a.h) apply_norm<NV, WPR, VEC>(h, a.post, a.post_w, a.post_b, C, a.eps, c0, red, warp, lane);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * WPR * 256;
         if (c >= C) continue;
         if (a.h && a.gate) {
-            if (!kEarly) load8<T, VEC>(a.gate + g * a.ldgate, c, C, gt);
+            if (NV > 1) load8<T, VEC>(a.gate + g * a.ldgate, c, C, gt);
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[i][j] *= gt[j];
         }
@@ -161,12 +166,12 @@ __global__ void __launch_bounds__(kThreads) few_kernel(BlockNormArgs<T> a, int64
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * WPR * 256;
         if (a.scale && c < C) {
-            if (!kEarly) load8<T, VEC>(a.scale + g * a.ldmod, c, C, sc);
+            if (!EARLY) load8<T, VEC>(a.scale + g * a.ldmod, c, C, sc);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[i][j] *= 1.0f + sc[j];
         }
         if (a.shift && c < C) {
-            if (!kEarly) load8<T, VEC>(a.shift + g * a.ldmod, c, C, sh);
+            if (!EARLY) load8<T, VEC>(a.shift + g * a.ldmod, c, C, sh);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[i][j] += sh[j];
         }
@@ -267,7 +272,7 @@ __device__ __forceinline__ void cut(F8& f, int c, int C) {
 // CTAs per SM that the registers are cut for. More rows in flight are worth some spilling at fp16 ([189809 x 1024] 299 us
 // with 2, 273 with 3; 512 columns 154 with 3, 142 with 4), not at fp32 (1024 columns 553 with 2, 680 with 3).
 template <class T> constexpr int rows_ctas(int nv, bool perrow) {
-    if (nv == 4) return sizeof(T) == 2 && !perrow ? 3 : 2;
+    if (nv >= 3) return sizeof(T) == 2 && !perrow ? 3 : 2;
     return (perrow ? 4 : sizeof(T) == 2 ? 6 : 5) - nv;
 }
 
@@ -275,9 +280,16 @@ template <class T> constexpr int rows_ctas(int nv, bool perrow) {
 // columns per lane. Shared memory: four vectors, A1, B1, A2, B2 of the modulation's rows (the range is cut where
 // that changes), or with PERROW (a modulation per row or few rows, loaded with the row) the norms' weights and
 // biases; each as the first and the second four of the lanes' eights, so that a warp reads 512 consecutive bytes.
+// Threads of a CTA. Eight warps per row: its vectors (96 KB with three per lane, 128 KB with four) are shared by two rows,
+// or three where the registers hold them ([20000 x 8192] fp16: 555 us with one row, 336 with two, 375 with three; 6000
+// columns 296 with two, 264 with three).
+template <class T> constexpr int rows_threads(int nv, int wpr, bool perrow) {
+    return wpr < 8 ? kThreads : nv == 3 && sizeof(T) == 2 && !perrow ? 768 : 512;
+}
 template <class T, int NV, int LPR, int WPR, bool PERROW>
-__global__ void __launch_bounds__(kThreads, rows_ctas<T>(NV, PERROW))
+__global__ void __launch_bounds__(rows_threads<T>(NV, WPR, PERROW), WPR == 8 ? 1 : rows_ctas<T>(NV, PERROW))
     rows_kernel(BlockNormArgs<T> a, int64_t ktiles, int64_t per) {
+    constexpr int kThreads = rows_threads<T>(NV, WPR, PERROW), kWarps = kThreads / 32;
     constexpr int kLanes = LPR * WPR, kRows = kThreads / kLanes;  // lanes per row, rows at a time
     constexpr int kVecs = NV * kLanes;                             // vectors of 8 columns per row
     extern __shared__ float4 fold[];                               // [4][2][kVecs]
@@ -482,14 +494,23 @@ template <class T, int NV, int WPR> void launch(const BlockNormArgs<T>& a, bool 
     const int64_t grid = (a.rows + kWarps / WPR - 1) / (kWarps / WPR);
     if (grid > INT32_MAX) fail(kUnsupported, "block_norm: too many rows for one launch");
     const int64_t kt = mx4::k_tiles(a.C);
-    if (vec) few_kernel<T, NV, WPR, true><<<unsigned(grid), kThreads, 0, s>>>(a, kt);
-    else few_kernel<T, NV, WPR, false><<<unsigned(grid), kThreads, 0, s>>>(a, kt);
+    auto go = [&](auto v, auto early) {
+        few_kernel<T, NV, WPR, decltype(v)::value, decltype(early)::value><<<unsigned(grid), kThreads, 0, s>>>(a, kt);
+    };
+    const bool early = NV == 1 && grid <= 4 * device_sm_count();  // one wave of CTAs
+    if constexpr (NV == 1) {
+        if (early && vec) go(std::true_type(), std::true_type());
+        else if (early) go(std::false_type(), std::true_type());
+    }
+    if (!early && vec) go(std::true_type(), std::false_type());
+    else if (!early) go(std::false_type(), std::false_type());
     VB_LAUNCH();
 }
 
 template <class T, int NV, int LPR, int WPR, bool PERROW> void launch_rows(const BlockNormArgs<T>& a, cudaStream_t s) {
-    constexpr int kSmem = 4 * 2 * NV * LPR * WPR * int(sizeof(float4)), kRows = kThreads / (LPR * WPR);
-    static_assert(kSmem <= 65536, "vectors of one row");
+    constexpr int kThreads = rows_threads<T>(NV, WPR, PERROW), kRows = kThreads / (LPR * WPR);
+    constexpr int kSmem = 4 * 2 * NV * LPR * WPR * int(sizeof(float4));
+    static_assert(kSmem <= 131072, "vectors of one row");
     static std::atomic<int> per_sm[64];  // resident CTAs per SM, by device
     auto* kernel = &rows_kernel<T, NV, LPR, WPR, PERROW>;
     int dev = 0, n = 0;
@@ -523,11 +544,11 @@ template <class T> void block_norm(const BlockNormArgs<T>& a, cudaStream_t s) {
     // a warp per row once the rows fill the SMs' warps; with fewer rows, as many warps per row as it has
     // 256-column pieces, for latency
     // rows_kernel from the rows on where it is the faster one ([2000 x 1024] fp16, vectors folded: 9.7 -> 8.0 us, and
-    // [9000 x 1024] 39 -> 22; a modulation per row: [5000 x 1024] fp16 32 -> 27, but [2562 x 1000] fp32 19 -> 29, for want of
+    // [9000 x 1024] 39 -> 22; a modulation per row: [5000 x 1024] fp16 32 -> 27, but [2562 x 1000] fp32 17 -> 29, for want of
     // registers). Folding one modulation takes a CTA the time of some 50 rows
     const bool fold = !a.group || a.group >= 1024 || (!a.gate && !a.scale && !a.shift);
     constexpr bool kPerRow = sizeof(T) == 2;
-    if (vec && nv <= 16 && (fold || kPerRow) && a.rows >= int64_t(fold ? 4 : 8) * device_sm_count()) {
+    if (vec && nv <= 32 && (fold || kPerRow) && a.rows >= int64_t(fold ? 4 : 8) * device_sm_count()) {
         auto go = [&](auto n, auto lanes, auto warps) {
             constexpr int kN = decltype(n)::value, kL = decltype(lanes)::value, kW = decltype(warps)::value;
             if constexpr (kPerRow) {
@@ -537,15 +558,24 @@ template <class T> void block_norm(const BlockNormArgs<T>& a, cudaStream_t s) {
         };
         std::integral_constant<int, 1> one;
         std::integral_constant<int, 2> n2;
+        std::integral_constant<int, 3> n3;
         std::integral_constant<int, 4> n4;
+        std::integral_constant<int, 8> n8;
         std::integral_constant<int, 32> warp;
+        // three vectors per lane rather than four that are not full ([40000 x 768] fp16: 53 against 66 us, [20000 x 2800] 115
+        // against 159, fp32 175 against 194; but [40000 x 768] fp32 92 against 83)
         if (a.C <= 64) go(one, std::integral_constant<int, 8>(), one);
         else if (a.C <= 128) go(one, std::integral_constant<int, 16>(), one);
         else if (nv <= 1) go(one, warp, one);
         else if (nv <= 2) go(n2, warp, one);
+        else if (nv <= 3 && sizeof(T) == 2) go(n3, warp, one);
         else if (nv <= 4) go(n4, warp, one);
+        else if (nv <= 6) go(n3, warp, n2);
         else if (nv <= 8) go(n4, warp, n2);
-        else go(n4, warp, n4);
+        else if (nv <= 12) go(n3, warp, n4);
+        else if (nv <= 16) go(n4, warp, n4);
+        else if (nv <= 24) go(n3, warp, n8);
+        else go(n4, warp, n8);
         return;
     }
     if (nv == 1) return launch<T, 1, 1>(a, vec, s);
