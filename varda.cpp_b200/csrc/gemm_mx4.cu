@@ -30,12 +30,14 @@
 // 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us with a bias), the same with A's
 // rows kept in shared memory (533), plain stores instead of TMA stores (517).
 //
-// Every wait is bounded as in gemm_tc.cu: on timeout a CTA sets the device error flag, stops issuing, waits for
-// its own copies and MMAs in flight, frees its tensor memory and returns.
+// Every wait is bounded: when one runs out a CTA sets the device error flag, stops issuing, waits for its own copies and
+// MMAs in flight, frees its tensor memory and returns. All lanes of a warp wait and act on one answer, as what follows
+// needs the whole warp (tensor-memory loads and stores, __syncwarp).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <mutex>
 #include <string>
 
@@ -71,20 +73,27 @@ struct Params {
     int64_t ktiles_out;
     int M, N, K64;  // K64: MMAs along K, ceil(K / 64)
     int gelu_tanh;
+    unsigned long long wait_ns;  // limit of each wait
+    int withhold;                // test hook: block 0 never loads its first stage
 };
 
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
     if (mbar_test(b, parity)) return true;
     const uint64_t t0 = now_ns();
     for (;;) {
         if (mbar_test(b, parity)) return true;
         if (*abort_flag) return false;
-        if (now_ns() - t0 > kTimeoutNs) {
+        if (now_ns() - t0 > limit_ns) {
             *abort_flag = 1;
             atomicExch(&g_error, 1);
             return false;
         }
     }
+}
+// Bounded wait of a whole warp, with one answer for it: false if any lane gave up (the lanes' clocks, flags and barrier
+// may change between one lane's last look and another's).
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
+    return __all_sync(kFull, lane_wait(b, parity, abort_flag, limit_ns));
 }
 // Ignores the abort flag (to drain work in flight), still bounded.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
@@ -277,29 +286,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool leader = elect_one();
             int stage = 0;
             uint32_t phase = 0;
-            for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
+            bool ok = true, withhold = p.withhold && blockIdx.x == 0;
+            for (int tile = unit0; ok && tile < tiles; tile += units) {
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) break;
-                    if (leader) {
+                    ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_ns);
+                    if (!ok) break;
+                    if (leader && !withhold) {
                         if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * (L::kA + L::kB)));
                         load_codes<PAIR>(sA + stage * L::kA, &tmA, &full[stage], kb * BKB, mb * UM + int(rank) * BM);
                         load_codes<PAIR>(sB + stage * L::kB, &tmW, &full[stage], kb * BKB, nb * BN + int(rank) * (BN / 2));
                     }
                     __syncwarp();
+                    withhold = false;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
             }
-            if (*abort_flag) settle();
         } else if (warp == 2) {
             // ---------------- TMA producer of the scales (all of the W tile's, in both CTAs of a pair)
             const bool leader = elect_one();
             int slot = 0;
             uint32_t phase = 0;
-            for (int tile = unit0; tile < tiles && !*abort_flag; tile += units) {
+            bool ok = true;
+            for (int tile = unit0; ok && tile < tiles; tile += units) {
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&sempty[slot], phase ^ 1, abort_flag)) break;
+                    ok = mbar_wait(&sempty[slot], phase ^ 1, abort_flag, p.wait_ns);
+                    if (!ok) break;
                     if (leader) {
                         mbar_expect_tx(&sfull[slot], uint32_t(L::kSA + L::kSB));
                         uint8_t* d = sSc + slot * (L::kSA + L::kSB);
@@ -310,7 +323,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (++slot == SLOTS) slot = 0, phase ^= 1;
                 }
             }
-            if (*abort_flag) settle();
         } else if (warp == 1 && rank == 0) {
             // ---------------- MMA issuer (the pair's leader issues for both CTAs). The whole warp runs the loop and one
             // lane issues, so that descriptors and addresses are uniform values
@@ -320,14 +332,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t phase = 0;
             bool any = false;
             for (int tile = unit0; tile < tiles; tile += units, ++it) {
-                if (*abort_flag) break;
                 const int ab = it & 1;
                 // the accumulator has been read: its own last tile's, or (overlapping accumulators) the
                 // previous tile's, whose readers were done with the tile before
                 if (L::kOverlap) {
-                    if (it > 0 && !mbar_wait(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag)) break;
+                    if (it > 0 && !mbar_wait(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag, p.wait_ns)) break;
                 } else {
-                    if (!mbar_wait(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag)) break;
+                    if (!mbar_wait(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) break;
                 }
                 fence_after();
                 const uint32_t d = tmem + uint32_t(ab * L::kAcc1);
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t half = BN == 64 ? uint32_t((tile % n_n) & 1) * 2u : 0u;
                 bool ok = true;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag)) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.wait_ns)) {
                         ok = false;
                         break;
                     }
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int tile = unit0; ok && tile < tiles; tile += units) {
             for (int kb = 0; kb < kblocks; ++kb) {
-                if (!mbar_wait(&sfull[slot], sphase, abort_flag)) {
+                if (!mbar_wait(&sfull[slot], sphase, abort_flag, p.wait_ns)) {
                     ok = false;
                     break;
                 }
@@ -394,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int t = 0; t < L::kNTiles; ++t) v[j][1 + t] = *reinterpret_cast<const uint4*>(src + L::kSA + (2 * t + j) * 512);
                 }
-                if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {  // the MMAs that read this buffer are done
+                if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_ns)) {  // the MMAs that read this buffer are done
                     ok = false;
                     break;
                 }
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = lane; i < L::kCW; i += 32) wb[i] = bias && colw + i < p.N ? to_f<T>(__ldg(bias + colw + i)) : 0.0f;
             __syncwarp();
-            if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag)) {
+            if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag, p.wait_ns)) {
                 if (EPI == k::kEpiResidual && lane == 0) mbar_drain(rbar, rphase);
                 break;
             }
@@ -523,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (lane == 0) load_residual(col0, row0);
                         }
                         if (L::kSW == 32 || c == 0) {
-                            if (!mbar_wait(rbar, rphase, abort_flag)) {
+                            if (!mbar_wait(rbar, rphase, abort_flag, p.wait_ns)) {
                                 if (lane == 0) mbar_drain(rbar, rphase);
                                 __syncwarp();
                             }
@@ -590,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_before();
     __syncthreads();
+    if (*abort_flag) settle();  // (every thread, once no warp issues any more)
     if (PAIR) cluster_sync();  // no CTA leaves while its peer may still read its shared memory or signal it
     if (warp == 3) {
         fence_after();
@@ -640,8 +652,12 @@ template <class T, int BN, bool PAIR, int EPI, bool OUT4> void launch(const Gemm
         ty = rows_map(a.Y, a.M, a.N, a.ldy, L::kSW);
         if (EPI == k::kEpiResidual) tr = rows_map(a.R, a.M, a.N, a.ldr, L::kSW);
     }
+    // failure-path test hooks (host side, no fault): VB_DEBUG_WAIT_NS shortens every wait's limit and
+    // VB_DEBUG_MX4_WITHHOLD=1 makes block 0 skip its first stage's codes, so that the waits on them run out
+    const char* wn = std::getenv("VB_DEBUG_WAIT_NS");
+    const char* wh = std::getenv("VB_DEBUG_MX4_WITHHOLD");
     const Params p{a.bias, a.Y, a.ldy, a.Yc, a.ldyc, a.Ys, k_tiles(a.N), int(a.M), int(a.N), int((a.K + 63) / 64),
-                   a.gelu_tanh ? 1 : 0};
+                   a.gelu_tanh ? 1 : 0, wn && *wn ? std::strtoull(wn, nullptr, 10) : kTimeoutNs, wh && *wh && std::atoi(wh) != 0};
     constexpr int UM = PAIR ? 2 * BM : BM;
     const int64_t tiles = ((a.M + UM - 1) / UM) * ((a.N + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) fail(kUnsupported, "gemm_mx4: too many output tiles");
