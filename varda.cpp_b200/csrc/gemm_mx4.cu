@@ -77,11 +77,13 @@ struct Params {
     int withhold;                // test hook: block 0 never loads its first stage
 };
 
+template <bool CL>
 __device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
-    if (mbar_test(b, parity)) return true;
+    auto test = [&] { return CL ? mbar_test_cl(b, parity) : mbar_test(b, parity); };
+    if (test()) return true;
     const uint64_t t0 = now_ns();
     for (;;) {
-        if (mbar_test(b, parity)) return true;
+        if (test()) return true;
         if (*abort_flag) return false;
         if (now_ns() - t0 > limit_ns) {
             *abort_flag = 1;
@@ -91,9 +93,10 @@ __device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile
     }
 }
 // Bounded wait of a whole warp, with one answer for it: false if any lane gave up (the lanes' clocks, flags and barrier
-// may change between one lane's last look and another's).
+// may change between one lane's last look and another's). CL: the barrier also takes arrivals of the pair's other CTA.
+template <bool CL = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
-    return __all_sync(kFull, lane_wait(b, parity, abort_flag, limit_ns));
+    return __all_sync(kFull, lane_wait<CL>(b, parity, abort_flag, limit_ns));
 }
 // Ignores the abort flag (to drain work in flight), still bounded.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
@@ -126,9 +129,12 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
-// Arrival on a barrier of the pair that tells of tensor memory read or written: tcgen05.fence orders that, and
-// no other memory goes with it. (A release at cluster scope waits about 1000 cycles for the thread's other
-// writes: 1000 us instead of 450 on [189809 x 4096] x [4096 x 1024] then.)
+// Arrival on a barrier of the pair that tells of tensor memory read or written, and of nothing else: the order that the PTX
+// ISA gives in "tcgen05 memory consistency model", canonical synchronisation patterns, for an instruction and another
+// thread that needs its end: tcgen05.ld or st, tcgen05.wait, tcgen05.fence::before_thread_sync,
+// mbarrier.arrive.relaxed.cluster; there mbarrier.try_wait at cluster scope, tcgen05.fence::after_thread_sync,
+// tcgen05.mma (the fence orders what came before it with the arrival, an execution ordering instruction). A release at
+// cluster scope would also wait for the thread's other writes: 766 us instead of 445 on [189809 x 1024] x [1024 x 4096].
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -336,9 +342,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the accumulator has been read: its own last tile's, or (overlapping accumulators) the
                 // previous tile's, whose readers were done with the tile before
                 if (L::kOverlap) {
-                    if (it > 0 && !mbar_wait(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag, p.wait_ns)) break;
+                    if (it > 0 && !mbar_wait<PAIR>(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag, p.wait_ns)) break;
                 } else {
-                    if (!mbar_wait(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) break;
+                    if (!mbar_wait<PAIR>(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) break;
                 }
                 fence_after();
                 const uint32_t d = tmem + uint32_t(ab * L::kAcc1);
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t half = BN == 64 ? uint32_t((tile % n_n) & 1) * 2u : 0u;
                 bool ok = true;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.wait_ns)) {
+                    if (!mbar_wait<PAIR>(&full[stage], phase, abort_flag, p.wait_ns)) {
                         ok = false;
                         break;
                     }
