@@ -53,3 +53,29 @@ def test_waits_run_out_and_the_device_stays_usable(M, N, K, dt, epi, quant, monk
         t.blocks_check((codes, tiles), M, N, want, err)
     else:
         t.product_check(t.get(y).astype(float), A[2], W[2], bias, R, dt, epi)
+
+
+def test_a_timeout_beside_the_attention_s_is_not_lost(monkeypatch):
+    """Both kernels' waits run out before anyone asks: vb_check_device reports one, then the other, then none."""
+    import numpy as np
+    rng = np.random.default_rng(1)
+    n, C, heads = 300, 256, 4
+    src, dst = [], []
+    for i in range(n):
+        s = np.unique(np.clip(i + rng.integers(-20, 20, 6), 0, n - 1))
+        src += list(s)
+        dst += [i] * len(s)
+    rp, src, _, attr = vb.build_csr(np.array([src, dst], np.int64), rng.normal(size=(len(src), 3)).astype(np.float16).astype(np.float32), n, n)
+    tiles = vb.Tiles(rp, src, attr, n, C // heads, kind=vb.Tiles.TC)
+    q, k, v, xr, out = (torch.zeros(n, C, device="cuda", dtype=torch.float16) for _ in range(5))
+    M, N, K = TILES[0]
+    A, W, _, _ = t.product_case(M, N, K, vb.FP16, 2)
+    y = torch.zeros(M, N, device="cuda", dtype=torch.float16)
+    withhold(monkeypatch)
+    monkeypatch.setenv("VB_DEBUG_TC_WITHHOLD", "1")
+    tiles.attention(0, n, q, C, k, v, C, xr, C, out, C, torch.zeros(4, C, device="cuda"), C, heads, C // heads)
+    vb.gemm_mx4(vb.FP16, A[0], A[0].stride(0), A[1], W[0], W[0].stride(0), W[1], None, y, N, None, 0, M, N, K)
+    torch.cuda.synchronize()
+    timed_out("4-bit GEMM")
+    timed_out("attention")
+    vb.check_device()

@@ -222,9 +222,9 @@ int64_t vb_decoder_chunk_rows(const vb_model* m) { return m ? m->m->decoder_chun
 
 int vb_check_device(void) {
     return guard([&] {
-        const int mx4 = vb::mx4::take_error();  // (the engine has none of these GEMMs)
+        // one flag per call: each is cleared when it is reported
+        if (vb::mx4::take_error()) vb::fail(vb::kTimeout, "a device-side wait timed out in the 4-bit GEMM");
         device_errors();
-        if (mx4) vb::fail(vb::kTimeout, "a device-side wait timed out in the 4-bit GEMM");
     });
 }
 
