@@ -307,9 +307,10 @@ int vb_mx4_dequantize(int dtype, const void* codes, int64_t ldc, const void* sca
                       int64_t ldy, void* stream);
 
 /* vb_gemm on 4-bit blocks: Y[M, N] = A[M, K] W[N, K]^T (+ bias [N], may be NULL), then epilogue 0 = none, 1 =
- * GELU (gelu_tanh selects the tanh form), 2 = + residual R[M, N]; bias, Y and R of dtype. Sums in fp32,
- * rounded to dtype once, after the epilogue (vb_gemm rounds before its epilogue too). Y and R: 16-byte
- * aligned, rows (ldy, ldr >= N elements) a multiple of 16 bytes apart; R may be Y. lda, ldw in bytes. */
+ * GELU (gelu_tanh selects the tanh form; the other gives 0, its limit, for -Inf), 2 = + residual R[M, N]; bias,
+ * Y and R of dtype. Sums in fp32, rounded to dtype once, after the epilogue (vb_gemm rounds before its epilogue
+ * too). Y and R: 16-byte aligned, rows (ldy, ldr >= N elements) a multiple of 16 bytes apart; R may be Y. lda,
+ * ldw in bytes. */
 int vb_gemm_mx4(int dtype, const void* A, int64_t lda, const void* sA, const void* W, int64_t ldw, const void* sW,
                 const void* bias, void* Y, int64_t ldy, const void* R, int64_t ldr, int64_t M, int64_t N, int64_t K,
                 int epilogue, int gelu_tanh, void* stream);

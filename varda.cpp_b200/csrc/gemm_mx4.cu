@@ -43,6 +43,7 @@
 
 #include "common.h"
 #include "dev.cuh"
+#include "gelu.cuh"
 #include "gemm_mx4.cuh"
 #include "gemm_tc.cuh"
 #include "ptx.cuh"
@@ -175,25 +176,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
             "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
-}
-
-// GELU in fp32 with one special-function operation: x Phi(x) = max(x, 0) - z Phi(-z), z = |x|, and
-// Phi(-z) = 2^P(z) with P a polynomial fitted to log2 Phi(-z) on [0, 5.6] (weighted least squares towards the
-// smallest largest error of z Phi(-z)): |error| <= 3e-7, at most 5e-7 |x|. Past 5.6, z Phi(-z) stays at its
-// 6e-8. (gemm_tc.cu's form takes two: at 16 a clock and SM they alone make 345 us on [189809 x 1024] x [1024 x 4096].
-// Scalar instead of packed operations: 650 us there, against 587 then.)
-__device__ __forceinline__ float2 gelu2(float2 x) {
-    const float2 n = make_float2(fmaxf(-fabsf(x.x), -5.6f), fmaxf(-fabsf(x.y), -5.6f));
-    float2 p = __ffma2_rn(n, make_float2(3.26786503e-05f, 3.26786503e-05f), make_float2(7.58978247e-04f, 7.58978247e-04f));
-    p = __ffma2_rn(n, p, make_float2(8.02492630e-03f, 8.02492630e-03f));
-    p = __ffma2_rn(n, p, make_float2(5.32902256e-02f, 5.32902256e-02f));
-    p = __ffma2_rn(n, p, make_float2(-4.58889902e-01f, -4.58889902e-01f));
-    p = __ffma2_rn(n, p, make_float2(1.15115345f, 1.15115345f));
-    p = __ffma2_rn(n, p, make_float2(-9.99998868e-01f, -9.99998868e-01f));
-    float2 r;  // max(x, 0), NaN kept
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.x) : "f"(x.x));
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.y) : "f"(x.y));
-    return __ffma2_rn(n, make_float2(ex2f(p.x), ex2f(p.y)), r);
 }
 
 // T: type of bias, residual and output. OUT4: 4-bit output (T is the bias's type).
@@ -509,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float2 g = gelu2(make_float2(v[i], v[i + 1]));
+                            const float2 g = gelu2<kFineGelu<T> && !OUT4>(make_float2(v[i], v[i + 1]));
                             v[i] = g.x, v[i + 1] = g.y;
                         }
                     }

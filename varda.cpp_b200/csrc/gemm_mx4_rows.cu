@@ -11,6 +11,7 @@
 
 #include "common.h"
 #include "dev.cuh"
+#include "gelu.cuh"
 #include "gemm_mx4.cuh"
 
 namespace vb::mx4 {
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(GemmArgs<T> a) {
 #pragma unroll
     for (int i = 0; i < WK; ++i) y += part[gi * WK + i][lane];
     if (a.bias) y += to_f<T>(a.bias[n]);
-    if (a.epi == k::kEpiGelu) y = gelu(y, a.gelu_tanh);
+    if (a.epi == k::kEpiGelu) y = a.gelu_tanh ? gelu(y, true) : gelu2<kFineGelu<T>>(make_float2(y, y)).x;
     if (a.epi == k::kEpiResidual) y += to_f<T>(a.R[m * a.ldr + n]);
     a.Y[m * a.ldy + n] = from_f<T>(y);
 }
