@@ -1,4 +1,5 @@
-"""Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile.
+"""Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile,
+groups without a modulation.
 
 Tolerances as in test_mx4_gpu.py. GELU alone (a product of zeros and a bias x) is max(x, 0) - t, t = |x| Phi(-|x|) as
 |x| 2^P: 2^P within 2^-22 (ex2) and ln 2 times P's rounding, 2^-22 (1 + |P|), of itself, P's fit (2e-7 of t's largest
@@ -99,3 +100,68 @@ def test_gelu_alone_in_4_bits(M, N, K):
     far = keep & (x < -5.6)  # a block of the tail: at most 16 times its values, each then rounded by half of itself at most
     top = np.repeat([np.abs(y[32 * b:32 * b + 32]).max() for b in range(nb)], 32)[:N]
     assert (np.abs(v[far]) <= 24 * top[far] + 2.0 ** -126).all() and (v[keep & (x < -17)] == 0).all()
+
+
+# ------------------------------------------------------------------ groups, ends of rows
+
+def run_norm(dt, x, C, group, y4, **kw):
+    """vb_block_norm -> [x', y] or [x', codes, scale tiles] on the host."""
+    rows = x.shape[0]
+    out = torch.zeros(rows, C, device="cuda", dtype=t.tdt(dt))
+    if y4:
+        codes, tiles = t.mx4_space(rows, C)
+        vb.block_norm(dt, rows, C, x, C, out=out, ldo=C, y_codes=codes, ldc=codes.stride(0), y_scales=tiles, rows_per_group=group, **kw)
+        return [t.get(out), t.get(codes), t.get(tiles)]
+    y = torch.zeros(rows, C, device="cuda", dtype=t.tdt(dt))
+    vb.block_norm(dt, rows, C, x, C, out=out, ldo=C, y=y, ldy=C, rows_per_group=group, **kw)
+    return [t.get(out), t.get(y)]
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows,C", [(9, 100), (1300, 40), (1300, 1024), (1250, 2000)])
+@pytest.mark.parametrize("group", [1, 3, 1100])
+def test_groups_without_a_modulation(rows, C, group, dt):
+    """rows_per_group says nothing where nothing is modulated: the bits of rows_per_group = 0. A gate without h, scale and
+    shift without y, strides and a norm's weight without what they belong to are not read."""
+    rng = np.random.default_rng(rows + C)
+    x, h, _, _, _, w, b = t.norm_case(rows, C, dt, 1, rng)
+    f32 = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    kw = dict(post=1, post_w=f32(w[0]), post_b=f32(b[0]), pre=2, pre_w=f32(w[1]), pre_b=f32(b[1]))
+    d, e = t.put(x, dt), t.put(h, dt)
+    for y4 in (False, True):
+        for more in (dict(h=e, ldh=C), dict(gate=e, ldgate=C)):
+            for p, q in zip(run_norm(dt, d, C, group, y4, **kw, **more), run_norm(dt, d, C, 0, y4, **kw, **{**more, "gate": None})):
+                assert np.array_equal(p, q)
+    kw = dict(pre=2, pre_w=f32(w[1]))
+    for p, q in zip(run_norm(dt, d, C, group, False, **kw, ldh=C + 1, ldgate=C + 1, ldmod=C + 1, post=1, post_w=f32(np.ones(C + 1, np.float32))[1:]),
+                    run_norm(dt, d, C, 0, False, **kw)):
+        assert np.array_equal(p, q)
+    outs = []
+    for g, m in ((group, e), (0, None)):
+        out = torch.zeros(rows, C, device="cuda", dtype=t.tdt(dt))
+        vb.block_norm(dt, rows, C, d, C, h=e, ldh=C, post=1, out=out, ldo=C, scale=m, shift=m, ldmod=C, rows_per_group=g)
+        outs.append(t.get(out))
+    assert np.array_equal(*outs)
+
+
+def test_groups_without_a_modulation_cost_nothing():
+    """A group per row without a modulation takes no longer than none (three times it at most)."""
+    rows, C, dt = 20000, 1024, vb.FP16
+    x, h, y, out = (torch.randn(rows, C, device="cuda").half() for _ in range(4))
+    w = torch.ones(C, device="cuda")
+    s = torch.cuda.current_stream().cuda_stream
+
+    def best(group):
+        times = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                vb.block_norm(dt, rows, C, x, C, h=h, ldh=C, post=1, post_w=w, out=out, ldo=C, pre=1, pre_w=w, y=y, ldy=C,
+                              rows_per_group=group, stream=s)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert best(1) <= 3 * best(0)

@@ -533,7 +533,19 @@ bool aligned(const void* p, int64_t row_bytes = 0) {
 
 }  // namespace
 
-template <class T> void block_norm(const BlockNormArgs<T>& a, cudaStream_t s) {
+template <class T> void block_norm(const BlockNormArgs<T>& args, cudaStream_t s) {
+    // What is not read chooses nothing: a gate and a norm without h, a modulation and a norm without y, a norm's vectors
+    // without the norm, strides without their array, groups without a modulation
+    BlockNormArgs<T> a = args;
+    if (!a.h) a.gate = nullptr, a.post = kNormNone, a.ldh = 0;
+    if (!a.y && !a.yc) a.scale = a.shift = nullptr, a.pre = kNormNone;
+    if (a.post == kNormNone) a.post_w = a.post_b = nullptr;
+    if (a.pre == kNormNone) a.pre_w = a.pre_b = nullptr;
+    if (!a.gate) a.ldgate = 0;
+    if (!a.scale && !a.shift) a.ldmod = 0;
+    if (!a.gate && !a.scale && !a.shift) a.group = 0;
+    if (!a.out) a.ldo = 0;
+    if (!a.y) a.ldy = 0;
     if (a.rows <= 0) return;
     if (a.C < 1 || a.C > kBlockNormMaxC) fail(kUnsupported, "block_norm: " + std::to_string(a.C) + " columns (1 to 16384)");
     const int64_t z = sizeof(T);
@@ -546,7 +558,7 @@ template <class T> void block_norm(const BlockNormArgs<T>& a, cudaStream_t s) {
     // rows_kernel from the rows on where it is the faster one ([2000 x 1024] fp16, vectors folded: 9.7 -> 8.0 us, and
     // [9000 x 1024] 39 -> 22; a modulation per row: [5000 x 1024] fp16 32 -> 27, but [2562 x 1000] fp32 17 -> 29, for want of
     // registers). Folding one modulation takes a CTA the time of some 50 rows
-    const bool fold = !a.group || a.group >= 1024 || (!a.gate && !a.scale && !a.shift);
+    const bool fold = !a.group || a.group >= 1024;
     constexpr bool kPerRow = sizeof(T) == 2;
     if (vec && nv <= 32 && (fold || kPerRow) && a.rows >= int64_t(fold ? 4 : 8) * device_sm_count()) {
         auto go = [&](auto n, auto lanes, auto warps) {
