@@ -1,5 +1,5 @@
 """Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile,
-groups without a modulation.
+groups without a modulation, what is past the last column.
 
 Tolerances as in test_mx4_gpu.py. GELU alone (a product of zeros and a bias x) is max(x, 0) - t, t = |x| Phi(-|x|) as
 |x| 2^P: 2^P within 2^-22 (ex2) and ln 2 times P's rounding, 2^-22 (1 + |P|), of itself, P's fit (2e-7 of t's largest
@@ -165,3 +165,15 @@ def test_groups_without_a_modulation_cost_nothing():
         return min(times)
 
     assert best(1) <= 3 * best(0)
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("rows", [3, 1300])
+@pytest.mark.parametrize("C", [1, 40, 301])
+@pytest.mark.parametrize("pre", [0, 1, 2])
+def test_codes_past_the_last_column_are_zero(rows, C, pre, dt):
+    """... whatever the signs before it: res_scale < 0 and no h."""
+    x = np.random.default_rng(C).normal(size=(rows, C))
+    _, codes, tiles = run_norm(dt, t.put(x, dt), C, 0, True, res_scale=-1.0, pre=pre)
+    c = np.stack((codes & 15, codes >> 4), -1).reshape(rows, -1)
+    assert (c[:, C:] == 0).all()

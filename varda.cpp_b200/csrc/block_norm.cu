@@ -176,7 +176,12 @@ __global__ void __launch_bounds__(kThreads, NV == 8 ? 1 : NV == 4 ? 2 : NV == 2 
             for (int j = 0; j < 8; ++j) x[i][j] += sh[j];
         }
         if (a.y && c < C) store8<T, VEC>(a.y + r * a.ldy, c, C, x[i]);
-        if (a.yc) store_blocks<T, 32>(a, r, c, C, live, ktiles, x[i]);
+        if (a.yc) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j >= C) x[i][j] = 0.0f;  // (-0 by a negative res_scale, NaN by an infinite rstd)
+            store_blocks<T, 32>(a, r, c, C, live, ktiles, x[i]);
+        }
     }
 }
 
