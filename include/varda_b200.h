@@ -329,7 +329,8 @@ int vb_gemm_mx4_quant(int dtype, const void* A, int64_t lda, const void* sA, con
  * gate, scale, shift (each may be NULL): row r / rows_per_group of [groups, C] (rows_per_group 0: one row
  * for all), scale and shift ldmod apart. out (x') may be NULL or x; y may be NULL, x or h (with that one's
  * leading dimension, and not also out). y_codes with y_scales: y as 4-bit blocks instead (y must then be NULL;
- * ldc in bytes; quantised from fp32, without the rounding to T). At least one output. */
+ * ldc in bytes; quantised from fp32, without the rounding to T). At least one output. Where gate or 1 + scale
+ * is Inf, a norm's bias may make the result NaN (n w + b is formed factor by factor for many rows). */
 enum { VB_NORM_NONE = 0, VB_NORM_LAYER = 1, VB_NORM_RMS = 2 };
 typedef struct {
     int64_t rows, C;

@@ -1,4 +1,4 @@
-"""Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile,
+"""Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile, Inf,
 groups without a modulation, what is past the last column.
 
 Tolerances as in test_mx4_gpu.py. GELU alone (a product of zeros and a bias x) is max(x, 0) - t, t = |x| Phi(-|x|) as
@@ -100,6 +100,26 @@ def test_gelu_alone_in_4_bits(M, N, K):
     far = keep & (x < -5.6)  # a block of the tail: at most 16 times its values, each then rounded by half of itself at most
     top = np.repeat([np.abs(y[32 * b:32 * b + 32]).max() for b in range(nb)], 32)[:N]
     assert (np.abs(v[far]) <= 24 * top[far] + 2.0 ** -126).all() and (v[keep & (x < -17)] == 0).all()
+
+
+# ------------------------------------------------------------------ NaN and Inf
+
+@pytest.mark.parametrize("rows", [5, 1300])
+def test_block_norm_infinite_modulation_without_bias(rows):
+    """gate and 1 + scale of Inf times a value that is not zero are Inf, where no bias is multiplied with them."""
+    C, dt = 256, vb.FP32
+    rng = np.random.default_rng(rows)
+    x, h, g, sc, _, w, _ = t.norm_case(rows, C, dt, 1, rng)
+    g[0, 5], sc[0, 9] = np.inf, -np.inf
+    out, y = (torch.zeros(rows, C, device="cuda") for _ in range(2))
+    f32 = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    vb.block_norm(dt, rows, C, t.put(x, dt), C, h=t.put(h, dt), ldh=C, post=2, post_w=f32(w[0]), gate=t.put(g, dt), out=out, ldo=C)
+    vb.block_norm(dt, rows, C, t.put(x, dt), C, pre=2, pre_w=f32(w[1]), scale=t.put(sc, dt), y=y, ldy=C)
+    with np.errstate(invalid="ignore"):
+        want_x, want_y = x + g * ref.norm(h, 2, w[0], None, 1e-5)[0], ref.norm(x, 2, w[1], None, 1e-5)[0] * (1 + sc)
+    for got, want in ((t.get(out), want_x), (t.get(y), want_y)):
+        assert np.array_equal(np.isinf(got), np.isinf(want)) and not np.isnan(got).any()
+        assert np.array_equal(np.sign(got[np.isinf(want)]), np.sign(want[np.isinf(want)]))
 
 
 # ------------------------------------------------------------------ groups, ends of rows

@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(rows_threads<T>(NV, WPR, PERROW), WPR == 8 ? 1
                 if (!PERROW && a.gate) {
                     load8<T, true>(a.gate + g * a.ldgate, c, C, m);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] *= m[j], b[j] *= m[j];
+                    for (int j = 0; j < 8; ++j) w[j] *= m[j], b[j] = a.post_b ? b[j] * m[j] : 0.0f;  // (0 Inf is no bias)
                 }
                 put(0);
             }
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(rows_threads<T>(NV, WPR, PERROW), WPR == 8 ? 1
             if (!PERROW && a.scale) {
                 load8<T, true>(a.scale + g * a.ldmod, c, C, m);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] *= 1.0f + m[j], b[j] *= 1.0f + m[j];
+                for (int j = 0; j < 8; ++j) w[j] *= 1.0f + m[j], b[j] = a.pre_b ? b[j] * (1.0f + m[j]) : 0.0f;
             }
             if (!PERROW && a.shift) {
                 load8<T, true>(a.shift + g * a.ldmod, c, C, m);
