@@ -1,5 +1,6 @@
 """Edges of the 4-bit product and the block norm on the B200: GELU's tails on every tile, Inf,
-groups without a modulation, what is past the last column.
+groups without a modulation, what is past the last column,
+narrow rows.
 
 Tolerances as in test_mx4_gpu.py. GELU alone (a product of zeros and a bias x) is max(x, 0) - t, t = |x| Phi(-|x|) as
 |x| 2^P: 2^P within 2^-22 (ex2) and ln 2 times P's rounding, 2^-22 (1 + |P|), of itself, P's fit (2e-7 of t's largest
@@ -197,3 +198,17 @@ def test_codes_past_the_last_column_are_zero(rows, C, pre, dt):
     _, codes, tiles = run_norm(dt, t.put(x, dt), C, 0, True, res_scale=-1.0, pre=pre)
     c = np.stack((codes & 15, codes >> 4), -1).reshape(rows, -1)
     assert (c[:, C:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", [vb.FP16, vb.FP32])
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 5, 9, 11])
+@pytest.mark.parametrize("group", [0, 1])
+def test_block_norm_of_narrow_rows(C, group, dt):
+    """Many rows of a few columns, the last vector of a row reaching into the next."""
+    rows, ld = 1300, -(-C // 4) * 4 if dt == vb.FP32 else -(-C // 8) * 8
+    rng = np.random.default_rng(C)
+    groups = rows if group else 1
+    at = np.arange(rows) if group else np.zeros(rows, int)
+    x, h, g, sc, sh, w, b = t.norm_case(rows, C, dt, groups, rng)
+    got = t.norm_run(x, h, 1, w[0], b[0], g, 0.75, 2, w[1], b[1], sc, sh, group, dt, ld)
+    t.norm_check(*got, x, h, 1, w[0], b[0], g[at], 0.75, 2, w[1], b[1], sc[at], sh[at], dt)

@@ -245,9 +245,13 @@ template <> struct Raw8<float> {
         if (n & 1) p[n & 6] = n & 2 ? q.z : q.x;
     }
 };
+// Whether the last vector of a row before the last may be read whole: rows start 16-byte aligned, so eight values from a
+// multiple of 8 below C end within the row's stride (fp16) or at most 4 values into the next row (fp32), which has them
+// if C is at least 4.
+template <class T> __device__ __forceinline__ bool reads_on(int C) { return sizeof(T) == 2 || C >= 4; }
 // Eight values from column c of a row of C; `more`: another row follows in memory, so that the row's last vector
-// can be read whole (rows start 16-byte aligned; what it holds past C is cut off later). Without one that vector is
-// left zero here, for last8 to fill: no else branch between a row's loads.
+// can be read whole (what it holds past C is cut off later). Without one that vector is left zero here, for last8
+// to fill: no else branch between a row's loads.
 template <class T> __device__ __forceinline__ Raw8<T> raw8(const T* row, int c, int C, bool more) {
     Raw8<T> r;
     r.zero();
@@ -394,7 +398,7 @@ __global__ void __launch_bounds__(rows_threads<T>(NV, WPR, PERROW), WPR == 8 ? 1
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[i].p[j] = __fmul2_rn(v[i].p[j], both(rstd));
             };
-            const bool more = r + 1 < a.rows;
+            const bool more = r + 1 < a.rows && reads_on<T>(a.C);
             Raw8<T> xr[NV], hr[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) xr[i] = raw8(a.x + r * a.ldx, col0 + i * kLanes * 8, C, more);
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(rows_threads<T>(NV, WPR, PERROW), WPR == 8 ? 1
             // PERROW: a lane's vectors of the modulation fly with the row
             Raw8<T> gr[NV], scr[NV], shr[NV];
             const int64_t gm = PERROW && a.group ? r / a.group : 0;
-            const bool more_g = PERROW && a.group && gm < (a.rows - 1) / a.group;
+            const bool more_g = PERROW && a.group && gm < (a.rows - 1) / a.group && reads_on<T>(a.C);
             if constexpr (PERROW) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
