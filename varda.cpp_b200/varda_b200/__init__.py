@@ -138,12 +138,24 @@ STEP = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.POINTER(ctypes.c_float), ctyp
 
 def _ptr(a):
     """The address of a device tensor or host array, for a c_void_p argument (None and integers are passed on)."""
-    if a is None or type(a) is int:
+    if a is None or isinstance(a, int):
         return a
     try:
         return a.data_ptr()  # torch tensor (device memory plumbing)
     except AttributeError:
         return a.ctypes.data_as(ctypes.c_void_p)
+
+
+def _addr(a):
+    """The same as an integer, 0 for None, to be packed into a struct."""
+    if a is None:
+        return 0
+    if isinstance(a, int):
+        return a
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        return a.ctypes.data
 
 
 def _check_out(a, n, what):
@@ -454,10 +466,10 @@ def block_norm(dtype, rows, C, x, ldx, h=None, ldh=0, post=NORM_NONE, post_w=Non
                rows_per_group=0, y=None, ldy=0, y_codes=None, ldc=0, y_scales=None, eps=1e-5, stream=None):
     """vb_block_norm: x' = res_scale x + gate * post(h) to `out`, pre(x') (1 + scale) + shift to `y` or, as 4-bit
     blocks, to `y_codes` and `y_scales`."""
-    a = BLOCK_NORM_ARGS.pack(rows, C, _ptr(x) or 0, ldx, _ptr(h) or 0, ldh, _ptr(post_w) or 0, _ptr(post_b) or 0,
-                             _ptr(gate) or 0, ldgate, _ptr(out) or 0, ldo, _ptr(pre_w) or 0, _ptr(pre_b) or 0,
-                             _ptr(scale) or 0, _ptr(shift) or 0, ldmod, rows_per_group, _ptr(y) or 0, ldy,
-                             _ptr(y_codes) or 0, ldc, _ptr(y_scales) or 0, post, pre, res_scale, eps)
+    a = BLOCK_NORM_ARGS.pack(rows, C, _addr(x), ldx, _addr(h), ldh, _addr(post_w), _addr(post_b),
+                             _addr(gate), ldgate, _addr(out), ldo, _addr(pre_w), _addr(pre_b),
+                             _addr(scale), _addr(shift), ldmod, rows_per_group, _addr(y), ldy,
+                             _addr(y_codes), ldc, _addr(y_scales), post, pre, res_scale, eps)
     check(lib.vb_block_norm(dtype, a, stream))
 
 
