@@ -93,7 +93,8 @@ constexpr int kLnNone = 0, kLnStats = 1, kLnFold = 2;
 constexpr int kMaxSegs = 16;  // records per row a folded GEMM reads (C <= 2048)
 
 // Bounded wait for the phase of parity `parity`. Returns false on timeout (after raising the CTA's
-// abort flag and the device error flag) or when another role already aborted.
+// abort flag and the device error flag) or when another role already aborted. Each lane gets its own answer: a warp
+// that goes on to warp-wide instructions votes on it.
 template <bool CL = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
     auto test = [&] { return CL ? mbar_test_cl(b, parity) : mbar_test(b, parity); };
@@ -237,7 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto next_tile = [&](int it, bool warp_wide) -> int {
         if (!dyn) return unit0 + it * units;
         const int slot = it % kRing;
-        if (!mbar_wait<true>(&rfull[slot], uint32_t(it / kRing) & 1u, abort_flag)) return -1;
+        const bool ok = mbar_wait<true>(&rfull[slot], uint32_t(it / kRing) & 1u, abort_flag);
+        if (warp_wide ? !__all_sync(d::kFull, ok) : !ok) return -1;
         const int t = ring[slot];
         if (warp_wide) __syncwarp();
         if (!warp_wide || lane == 0) {
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // kLnStats: this half row's segment record, from its first stored value
             float2 s1 = make_float2(0.0f, 0.0f), s2 = make_float2(0.0f, 0.0f);
             float kshift = 0.0f;
-            if (!mbar_wait(&tfull[ab], ap, abort_flag)) break;
+            if (!__all_sync(d::kFull, mbar_wait(&tfull[ab], ap, abort_flag))) break;
             fence_after();
             const uint32_t taddr = tmem + (uint32_t(lg * 32) << 16) + uint32_t(ab * BN + half * (BN / 2));
             bool ok = true, released = false;
