@@ -294,6 +294,7 @@ int vb_add_layernorm(int dtype, const void* a, const void* r, void* out1, const 
  *           be 255 (the functions here write 0); those of rows past the last are not used.
  * The same dtype, stream and error rules as above; nothing is allocated and there is no workspace, so calls may
  * be captured and may overlap. Outputs must not overlap inputs but where that is said. */
+/* (0 for sizes that the functions below refuse: under 1, or over 2^30 - 1) */
 int64_t vb_mx4_row_bytes(int64_t K);
 int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K);
 

@@ -1,4 +1,4 @@
-"""Addresses as the Python binding takes them (nothing is launched)."""
+"""Addresses and sizes as the Python binding takes them (nothing is launched)."""
 import ctypes
 import enum
 
@@ -40,4 +40,14 @@ def test_block_norm_takes_what_the_others_take(x, monkeypatch):
     monkeypatch.undo()
     with pytest.raises(vb.VardaError) as e:
         vb.block_norm(vb.FP16, 4, 64, x, 63, y=x, ldy=64)
+    assert e.value.code == 1
+
+
+@pytest.mark.parametrize("n", [1 << 30, (1 << 31) + 1, (1 << 63) - 1])
+def test_sizes_that_no_function_takes(n):
+    """No size for what quantise and product refuse, and no overflow on the way to it."""
+    assert vb.mx4_row_bytes(n) == 0 and vb.mx4_scale_bytes(n, 64) == 0 and vb.mx4_scale_bytes(64, n) == 0
+    assert vb.mx4_row_bytes((1 << 30) - 1) == 1 << 29
+    with pytest.raises(vb.VardaError) as e:
+        vb.mx4_quantize(vb.FP16, 1 << 20, n, 4, n, 1 << 20, 1 << 40, 1 << 20)
     assert e.value.code == 1

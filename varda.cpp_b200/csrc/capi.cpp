@@ -696,8 +696,10 @@ void check_blocks(const void* codes, int64_t ldc, const void* scales, int64_t K,
 
 }  // namespace
 
-int64_t vb_mx4_row_bytes(int64_t K) { return K > 0 ? vb::mx4::row_bytes(K) : 0; }
-int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K) { return rows > 0 && K > 0 ? vb::mx4::scale_bytes(rows, K) : 0; }
+int64_t vb_mx4_row_bytes(int64_t K) { return K > 0 && K <= kMaxDim ? vb::mx4::row_bytes(K) : 0; }
+int64_t vb_mx4_scale_bytes(int64_t rows, int64_t K) {
+    return rows > 0 && rows <= kMaxDim && K > 0 && K <= kMaxDim ? vb::mx4::scale_bytes(rows, K) : 0;
+}
 
 int vb_mx4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, void* codes, int64_t ldc, void* scales,
                     void* stream) {
