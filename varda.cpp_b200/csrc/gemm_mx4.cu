@@ -31,8 +31,11 @@
 // rows kept in shared memory (533), plain stores instead of TMA stores (517).
 //
 // Every wait is bounded: when one runs out a CTA sets the device error flag, stops issuing, waits for its own copies and
-// MMAs in flight, frees its tensor memory and returns. All lanes of a warp wait and act on one answer, as what follows
-// needs the whole warp (tensor-memory loads and stores, __syncwarp).
+// MMAs in flight, frees its tensor memory and returns. Each lane of a warp waits for itself, and the barrier may complete
+// or the time run out between two lanes' looks; so no lane leaves a loop by its own answer. Lanes that gave up take part in
+// the warp's instructions (tensor memory read or written in vain), and the warp votes where it has to meet anyway, before
+// anything is handed on ([189809 x 256] x [256 x 4096] 276 us, as with lanes that left by themselves; with a vote at each
+// wait 284; the votes left cost [189809 x 4096] x [4096 x 1024] + residual 2%).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -78,8 +81,9 @@ struct Params {
     int withhold;                // test hook: block 0 never loads its first stage
 };
 
-template <bool CL>
-__device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
+// Bounded wait; false if this lane gave up. CL: the barrier also takes arrivals of the pair's other CTA.
+template <bool CL = false>
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
     auto test = [&] { return CL ? mbar_test_cl(b, parity) : mbar_test(b, parity); };
     if (test()) return true;
     const uint64_t t0 = now_ns();
@@ -93,12 +97,7 @@ __device__ __forceinline__ bool lane_wait(uint64_t* b, uint32_t parity, volatile
         }
     }
 }
-// Bounded wait of a whole warp, with one answer for it: false if any lane gave up (the lanes' clocks, flags and barrier
-// may change between one lane's last look and another's). CL: the barrier also takes arrivals of the pair's other CTA.
-template <bool CL = false>
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
-    return __all_sync(kFull, lane_wait<CL>(b, parity, abort_flag, limit_ns));
-}
+__device__ __forceinline__ bool whole_warp(bool ok) { return __all_sync(kFull, ok); }
 // Ignores the abort flag (to drain work in flight), still bounded.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
     const uint64_t t0 = now_ns();
@@ -279,13 +278,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_ns);
-                    if (!ok) break;
-                    if (leader && !withhold) {
+                    if (leader && ok && !withhold) {
                         if (rank == 0) mbar_expect_tx(&full[stage], uint32_t((PAIR ? 2 : 1) * (L::kA + L::kB)));
                         load_codes<PAIR>(sA + stage * L::kA, &tmA, &full[stage], kb * BKB, mb * UM + int(rank) * BM);
                         load_codes<PAIR>(sB + stage * L::kB, &tmW, &full[stage], kb * BKB, nb * BN + int(rank) * (BN / 2));
                     }
-                    __syncwarp();
+                    ok = whole_warp(ok);
+                    if (!ok) break;
                     withhold = false;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
@@ -300,14 +299,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int mb = tile / n_n, nb = tile - mb * n_n;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = mbar_wait(&sempty[slot], phase ^ 1, abort_flag, p.wait_ns);
-                    if (!ok) break;
-                    if (leader) {
+                    if (leader && ok) {
                         mbar_expect_tx(&sfull[slot], uint32_t(L::kSA + L::kSB));
                         uint8_t* d = sSc + slot * (L::kSA + L::kSB);
                         tma_load_3d(d, &tmSA, &sfull[slot], 0, kb * 2, (mb * UM) / 128 + int(rank));
                         tma_load_3d(d + L::kSA, &tmSW, &sfull[slot], 0, kb * 2, nb * BN / 128);
                     }
-                    __syncwarp();
+                    ok = whole_warp(ok);
+                    if (!ok) break;
                     if (++slot == SLOTS) slot = 0, phase ^= 1;
                 }
             }
@@ -318,32 +317,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t idesc0 = instr_desc(UM, BN, 0), idesc2 = instr_desc(UM, BN, 2);
             int stage = 0, it = 0;
             uint32_t phase = 0;
-            bool any = false;
-            for (int tile = unit0; tile < tiles; tile += units, ++it) {
+            bool any = false, ok = true;
+            for (int tile = unit0; ok && tile < tiles; tile += units, ++it) {
                 const int ab = it & 1;
                 // the accumulator has been read: its own last tile's, or (overlapping accumulators) the
                 // previous tile's, whose readers were done with the tile before
-                if (L::kOverlap) {
-                    if (it > 0 && !mbar_wait<PAIR>(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag, p.wait_ns)) break;
-                } else {
-                    if (!mbar_wait<PAIR>(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) break;
-                }
+                if (!L::kOverlap) ok = mbar_wait<PAIR>(&tempty[ab], (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns);
+                else if (it > 0) ok = mbar_wait<PAIR>(&tempty[ab ^ 1], uint32_t((it - 1) >> 1) & 1u, abort_flag, p.wait_ns);
                 fence_after();
                 const uint32_t d = tmem + uint32_t(ab * L::kAcc1);
                 // a 64-column tile of W uses half of a tile of 128 rows' scales
                 const uint32_t half = BN == 64 ? uint32_t((tile % n_n) & 1) * 2u : 0u;
-                bool ok = true;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait<PAIR>(&full[stage], phase, abort_flag, p.wait_ns)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = ok && mbar_wait<PAIR>(&full[stage], phase, abort_flag, p.wait_ns);
                     fence_after();
                     const int n_mma = min(4, p.K64 - 4 * kb);
                     const uint64_t a0 = codes_desc(smem_u32(sA + stage * L::kA));
                     const uint64_t b0 = codes_desc(smem_u32(sB + stage * L::kB));
                     const uint32_t sf = tmem + uint32_t(L::kSf + stage * L::kSfBuf);
-                    if (leader) {
+                    if (leader && ok) {
+                        any = true;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const uint32_t sa = sf + uint32_t((j >> 1) * L::kSfHalf);
@@ -354,18 +347,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (PAIR) mma_commit_pair(&empty[stage]);
                         else mma_commit(&empty[stage]);
                     }
-                    __syncwarp();
-                    any = true;
+                    ok = whole_warp(ok);
+                    if (!ok) break;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
-                if (!ok) break;
-                if (leader) {
+                if (leader && ok) {
                     if (PAIR) mma_commit_pair(&tfull[ab]);
                     else mma_commit(&tfull[ab]);
                 }
                 __syncwarp();
             }
-            if (any && leader) {  // every MMA issued by this thread completes before the tensor memory is freed
+            if (any) {  // every MMA issued by this thread (the leader) completes before the tensor memory is freed
                 if (PAIR) mma_commit_pair_local(drain);
                 else mma_commit(drain);
                 mbar_drain(drain, 0);
@@ -380,10 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int tile = unit0; ok && tile < tiles; tile += units) {
             for (int kb = 0; kb < kblocks; ++kb) {
-                if (!mbar_wait(&sfull[slot], sphase, abort_flag, p.wait_ns)) {
-                    ok = false;
-                    break;
-                }
+                ok = mbar_wait(&sfull[slot], sphase, abort_flag, p.wait_ns);
                 // both halves (a cut last stage's second half may hold no columns of K: it is then not used)
                 const uint8_t* src = sSc + slot * (L::kSA + L::kSB) + lane * 16;
                 uint4 v[2][1 + L::kNTiles];
@@ -393,10 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int t = 0; t < L::kNTiles; ++t) v[j][1 + t] = *reinterpret_cast<const uint4*>(src + L::kSA + (2 * t + j) * 512);
                 }
-                if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_ns)) {  // the MMAs that read this buffer are done
-                    ok = false;
-                    break;
-                }
+                // the MMAs that read this buffer are done
+                ok = ok && mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_ns);
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
@@ -405,7 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         st_scales(tq + uint32_t(stage * L::kSfBuf + j * L::kSfHalf + 4 * t), v[j][t]);
                 wait_st();
                 fence_before();
-                __syncwarp();
+                ok = whole_warp(ok);
+                if (!ok) break;
                 if (lane == 0) {
                     if (PAIR) mbar_arrive_peer(mapa(smem_u32(&full[stage]), 0));
                     else mbar_arrive(&full[stage]);
@@ -448,10 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = lane; i < L::kCW; i += 32) wb[i] = bias && colw + i < p.N ? to_f<T>(__ldg(bias + colw + i)) : 0.0f;
             __syncwarp();
-            if (!mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag, p.wait_ns)) {
-                if (EPI == k::kEpiResidual && lane == 0) mbar_drain(rbar, rphase);
-                break;
-            }
+            const bool ok = mbar_wait(&tfull[ab], uint32_t(it >> 1) & 1u, abort_flag, p.wait_ns);
             fence_after();
             const uint32_t taddr = tmem + (uint32_t(lg * 32) << 16) + uint32_t(ab * L::kAcc1 + grp * L::kCW);
             uint32_t acc[L::kCW / 32][32];
@@ -460,7 +445,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < L::kCW / 32; ++c) tmem_wait32(acc[c]);
             fence_before();
-            __syncwarp();
+            if (!whole_warp(ok)) {
+                if (EPI == k::kEpiResidual && lane == 0) mbar_drain(rbar, rphase);
+                break;
+            }
             if (lane == 0) {
                 if (PAIR) mbar_arrive_peer(ab ? te1 : te0);
                 else mbar_arrive(&tempty[ab]);
@@ -522,10 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (lane == 0) load_residual(col0, row0);
                         }
                         if (L::kSW == 32 || c == 0) {
-                            if (!mbar_wait(rbar, rphase, abort_flag, p.wait_ns)) {
-                                if (lane == 0) mbar_drain(rbar, rphase);
-                                __syncwarp();
-                            }
+                            if (!mbar_wait(rbar, rphase, abort_flag, p.wait_ns)) mbar_drain(rbar, rphase);  // (it is on its way)
                             rphase ^= 1;
                         }
 #pragma unroll
