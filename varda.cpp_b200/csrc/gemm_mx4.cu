@@ -97,7 +97,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
         }
     }
 }
-__device__ __forceinline__ bool whole_warp(bool ok) { return __all_sync(kFull, ok); }
+// The warp's vote, and a __syncwarp (which orders its memory accesses; the vote alone does not).
+__device__ __forceinline__ bool whole_warp(bool ok) {
+    ok = __all_sync(kFull, ok);
+    __syncwarp();
+    return ok;
+}
 // Ignores the abort flag (to drain work in flight), still bounded.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
     const uint64_t t0 = now_ns();
