@@ -23,12 +23,14 @@
 // second accumulator starts at column 128, over half of the first; since the epilogue reads all columns
 // at once, the next tile's MMAs start some 1300 cycles after the last one's end.
 //
-// What bounds it: [189809 x 1024] x [1024 x 4096] 442 us with a bias (1.55 GB of output, which alone takes 390 us to fill),
-// 545 with GELU (the epilogue: instruction issue 60%, special functions 38%, the fp32 pipe 42%), and
-// [189809 x 4096] x [4096 x 1024] + residual 365 us = 4360 TFLOP/s (tensor pipe 58%; the loads alone take 320 us, some
-// 10 TB/s from L2); run for seconds all of them are held by the 1 kW power limit (1.4 GHz: 420 us). Tried and dropped:
-// 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us with a bias), the same with A's
-// rows kept in shared memory (533), plain stores instead of TMA stores (517).
+// What bounds it, on [189809 x K] x [K x 4096] to fp16: at K = 64 the epilogue alone, 264 us with a bias (5.9 TB/s of
+// output), 410 with GELU (its arithmetic), and 446 with GELU and 4-bit output. At K = 1024, where the MMAs take some 240 by
+// themselves, 437, 539 and 540 to 575: the two do not overlap whole, as a tile's MMAs wait for the accumulator that they
+// share with the tile before, and the epilogue's warps, all in step, for the MMAs (issue slots 40 to 62% used, the tensor
+// pipe 33 to 43%; neither bounds it). Long sums: [189809 x 4096] x [4096 x 1024] + residual 369 us = 4320 TFLOP/s (tensor
+// pipe 55%; the loads alone take 320 us, some 10 TB/s from L2). Run for seconds all of them are held by the 1 kW power limit
+// (1.4 GHz: 440 us). Tried and dropped: 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us
+// with a bias), the same with A's rows kept in shared memory (533), plain stores instead of TMA stores (517).
 //
 // Every wait is bounded: when one runs out a CTA sets the device error flag, stops issuing, waits for its own copies and
 // MMAs in flight, frees its tensor memory and returns. Each lane of a warp waits for itself, and the barrier may complete
