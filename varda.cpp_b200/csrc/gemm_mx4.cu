@@ -29,7 +29,7 @@
 // share with the tile before, and the epilogue's warps, all in step, for the MMAs (issue slots 40 to 62% used, the tensor
 // pipe 33 to 43%; neither bounds it). Long sums: [189809 x 4096] x [4096 x 1024] + residual 369 us = 4320 TFLOP/s (tensor
 // pipe 55%; the loads alone take 320 us, some 10 TB/s from L2). Run for seconds all of them are held by the 1 kW power limit
-// (1.4 GHz: 440 us). Tried and dropped: 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us
+// (1.4 GHz: 445 us). Tried and dropped: 192-column tiles with two whole accumulators and two sets of epilogue warps (514 us
 // with a bias), the same with A's rows kept in shared memory (533), plain stores instead of TMA stores (517).
 //
 // Every wait is bounded: when one runs out a CTA sets the device error flag, stops issuing, waits for its own copies and
